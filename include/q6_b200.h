@@ -284,6 +284,92 @@ Q6_API int q6_sp_add_layernorm_gather_bf16(const uint16_t* x_local, const uint16
 Q6_API int q6_sp_barrier(uint32_t* const* signals, uint32_t* epoch, int world, int rank, int64_t timeout_ns,
                          q6_stream_t stream);
 
+/*
+ * Dense 16-bit linear and layer norm, forward and gradients: the trainable
+ * twins of the q6 linear's epilogue and of the block's modulate, over dense
+ * weights (a materialised image feed-forward, dense_img_ff_window.py:32-67).
+ * Tensors are passed untyped; `dtype` names their element type.  Row strides
+ * (ld*) are in elements and at least the row width; columns are contiguous.
+ */
+enum q6_dtype { Q6_DTYPE_BF16 = 0, Q6_DTYPE_F16 = 1, Q6_DTYPE_F32 = 2 };
+
+enum q6_activation {
+    Q6_ACT_NONE = 0,
+    Q6_ACT_GELU_TANH = 1, /* z sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3): GELU-tanh */
+    Q6_ACT_SILU = 2       /* z sigmoid(z) */
+};
+
+/*
+ * y = residual + gate * act(z),  z = x @ W^T + bias       (fp32 sums, one rounding)
+ *   x [M, K] (ldx), W [N, K] (ldw), bias [N], residual [M, N] (ldr), y [M, N] dense,
+ *   gate: row m takes vector m / rows_per_gate of gate [.., N] (ldg elements apart);
+ *   rows_per_gate divides M (M: one vector for all rows).
+ * bias, gate, residual may be null.  preact (nullable, [M, N] dense) receives z
+ * rounded to dtype, which q6_dense_linear_grad reads.  dtype: BF16 or F16.
+ * y may alias residual (same layout), nothing else may overlap an output.
+ * workspace: at least q6_dense_linear_workspace_bytes, 256-byte aligned.
+ */
+Q6_API int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* gate,
+                           int64_t ldg, int64_t rows_per_gate, const void* residual, int64_t ldr, void* y,
+                           void* preact, int64_t M, int64_t N, int64_t K, int dtype, int activation, void* workspace,
+                           size_t workspace_bytes, q6_stream_t stream);
+
+/* Operands that the tensor-core path copies to an aligned layout first: those
+   whose address is no multiple of 16 bytes or whose row stride is no multiple
+   of 8 elements. */
+enum q6_dense_pack { Q6_PACK_X = 1, Q6_PACK_W = 2, Q6_PACK_DY = 4 };
+
+Q6_API size_t q6_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int pack);
+
+/*
+ * Gradients of q6_dense_linear: with t = dy * gate and dz = t * act'(z),
+ *   dx = dz @ W [M, K],  dw = dz^T @ x [N, K],  dbias = sum_m dz [N],
+ *   dgate[s] = sum over the rows m of vector s of dy * act(z)   ([M / rows_per_gate, N]),
+ * each written only if its pointer is non-null, dense, in dtype (sums in fp32;
+ * dz is rounded to dtype as the operand of the two products).  The residual's
+ * gradient is dy itself.  preact is the forward's (may be null without an
+ * activation and without dgate).  x is read only for dw, W only for dx.
+ */
+Q6_API int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                const void* preact, const void* gate, int64_t ldg, int64_t rows_per_gate, void* dx,
+                                void* dw, void* dbias, void* dgate, int64_t M, int64_t N, int64_t K, int dtype,
+                                int activation, void* workspace, size_t workspace_bytes, q6_stream_t stream);
+
+/* Workspace of q6_dense_linear_grad; `outputs` holds Q6_GRAD_* of what is asked
+   for, `has_gate` whether gate is given, pack as above. */
+enum q6_dense_grad { Q6_GRAD_X = 1, Q6_GRAD_W = 2, Q6_GRAD_BIAS = 4, Q6_GRAD_GATE = 8 };
+
+Q6_API size_t q6_dense_linear_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t rows_per_gate,
+                                                   int activation, int has_gate, int outputs, int pack);
+
+/*
+ * y = xh * w + b,  xh = (x - mean(x)) * rstd,  rstd = 1 / sqrt(var(x) + eps)   over rows of D.
+ *   Row m takes vector v = m / rows_per_vec (a divisor of M) of weight / bias (ldv elements
+ *   apart, vec_dtype: dtype or F32; each may be null: w = 1, b = 0); with
+ *   Q6_NORM_ONE_PLUS the factor is 1 + weight (adaLN: weight = scale, bias = shift).
+ *   mean, rstd (fp32 [M], nullable together) receive the row statistics.
+ * x [M, D] (ldx), y [M, D] dense.  dtype: BF16, F16 or F32; statistics and sums in fp32.
+ */
+enum q6_norm_flags { Q6_NORM_ONE_PLUS = 1 };
+
+Q6_API int q6_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, int64_t ldv,
+                         int64_t rows_per_vec, void* y, float* mean, float* rstd, int64_t M, int64_t D, float eps,
+                         int dtype, int vec_dtype, int flags, q6_stream_t stream);
+
+/*
+ * Gradients of q6_layer_norm: with a = dy * w,
+ *   dx = rstd (a - mean(a) - xh mean(a xh)),
+ *   dweight[v] = sum over the rows of vector v of dy * xh,  dbias[v] = the same sum of dy
+ * (dense [M / rows_per_vec, D], vec_dtype).  dx, dweight, dbias may each be null.
+ * The row sums are taken in a fixed order: equal calls give equal bits.
+ */
+Q6_API int q6_layer_norm_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* weight, int64_t ldv,
+                              int64_t rows_per_vec, const float* mean, const float* rstd, void* dx, void* dweight,
+                              void* dbias, int64_t M, int64_t D, int dtype, int vec_dtype, int flags, void* workspace,
+                              size_t workspace_bytes, q6_stream_t stream);
+
+Q6_API size_t q6_layer_norm_grad_workspace_bytes(int64_t M, int64_t D, int64_t rows_per_vec, int dtype, int outputs);
+
 /* Device error word (0 = none, else a q6_error_site code).  Reading it
    synchronises the current device. */
 Q6_API int q6_get_device_error(int* code);

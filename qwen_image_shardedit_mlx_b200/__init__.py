@@ -6,6 +6,17 @@ weights (packed uint32 codes + bf16 per-group scale/bias), the reference's
 tcgen05 / CUDA-core kernels behind the C ABI in include/q6_b200.h.
 """
 
+from qwen_image_shardedit_mlx_b200.dense import (  # noqa: F401
+    dense_linear,
+    dense_linear_backward,
+    dense_linear_forward,
+    layer_norm,
+    layer_norm_backward,
+    layer_norm_forward,
+    layer_norm_modulate,
+    layer_norm_modulate_backward,
+    layer_norm_modulate_forward,
+)
 from qwen_image_shardedit_mlx_b200.ops import (  # noqa: F401
     clear_device_error,
     device_error,

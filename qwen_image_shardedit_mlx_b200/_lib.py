@@ -30,6 +30,25 @@ Q6_LORA_B_NMAJOR = 4
 Q6_SITE_PEER_BARRIER = 13
 Q6_SITE_SELFTEST = 64
 
+Q6_DTYPE_BF16 = 0
+Q6_DTYPE_F16 = 1
+Q6_DTYPE_F32 = 2
+
+Q6_ACT_NONE = 0
+Q6_ACT_GELU_TANH = 1
+Q6_ACT_SILU = 2
+
+Q6_PACK_X = 1
+Q6_PACK_W = 2
+Q6_PACK_DY = 4
+
+Q6_GRAD_X = 1
+Q6_GRAD_W = 2
+Q6_GRAD_BIAS = 4
+Q6_GRAD_GATE = 8
+
+Q6_NORM_ONE_PLUS = 1
+
 Q6_PATH_AUTO = 0
 Q6_PATH_SIMT = 1
 Q6_PATH_TENSOR = 2
@@ -65,6 +84,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "q6_add_layernorm_modulate_bf16": (_I, [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _F, _P]),
     "q6_qk_rmsnorm_rope_bf16": (_I, [_P, _I64, _I64, _I, _I, _P, _P, _P, _F, _P]),
     "q6_qk_rmsnorm_rope_joint_bf16": (_I, [_P, _I64, _I64, _I, _I, _P, _P, _P, _P, _I64, _I64, _I64, _F, _P]),
+    "q6_dense_linear": (
+        _I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _SZ, _P],
+    ),
+    "q6_dense_linear_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
+    "q6_dense_linear_grad": (
+        _I,
+        [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _SZ, _P],
+    ),
+    "q6_dense_linear_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I, _I, _I, _I]),
+    "q6_layer_norm": (_I, [_P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _F, _I, _I, _I, _P]),
+    "q6_layer_norm_grad": (
+        _I, [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _P, _SZ, _P],
+    ),
+    "q6_layer_norm_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I]),
     "q6_get_device_error": (_I, [ctypes.POINTER(ctypes.c_int)]),
     "q6_clear_device_error": (_I, []),
     "q6_last_path": (_I, []),
