@@ -304,15 +304,16 @@ enum q6_activation {
  *   x [M, K] (ldx), W [N, K] (ldw), bias [N], residual [M, N] (ldr), y [M, N] dense,
  *   gate: row m takes vector m / rows_per_gate of gate [.., N] (ldg elements apart);
  *   rows_per_gate divides M (M: one vector for all rows).
- * bias, gate, residual may be null.  preact (nullable, [M, N] dense) receives z
- * rounded to dtype, which q6_dense_linear_grad reads.  dtype: BF16 or F16.
+ * bias, gate, residual may be null.  preact (nullable, [M, N] dense, element type
+ * preact_dtype: dtype or F32) receives z, which q6_dense_linear_grad reads.
+ * dtype: BF16 or F16.
  * y may alias residual (same layout), nothing else may overlap an output.
  * workspace: at least q6_dense_linear_workspace_bytes, 256-byte aligned.
  */
 Q6_API int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* gate,
                            int64_t ldg, int64_t rows_per_gate, const void* residual, int64_t ldr, void* y,
-                           void* preact, int64_t M, int64_t N, int64_t K, int dtype, int activation, void* workspace,
-                           size_t workspace_bytes, q6_stream_t stream);
+                           void* preact, int preact_dtype, int64_t M, int64_t N, int64_t K, int dtype, int activation,
+                           void* workspace, size_t workspace_bytes, q6_stream_t stream);
 
 /* Operands that the tensor-core path copies to an aligned layout first: those
    whose address is no multiple of 16 bytes or whose row stride is no multiple
@@ -331,9 +332,10 @@ Q6_API size_t q6_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, i
  * activation and without dgate).  x is read only for dw, W only for dx.
  */
 Q6_API int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                const void* preact, const void* gate, int64_t ldg, int64_t rows_per_gate, void* dx,
-                                void* dw, void* dbias, void* dgate, int64_t M, int64_t N, int64_t K, int dtype,
-                                int activation, void* workspace, size_t workspace_bytes, q6_stream_t stream);
+                                const void* preact, int preact_dtype, const void* gate, int64_t ldg,
+                                int64_t rows_per_gate, void* dx, void* dw, void* dbias, void* dgate, int64_t M,
+                                int64_t N, int64_t K, int dtype, int activation, void* workspace,
+                                size_t workspace_bytes, q6_stream_t stream);
 
 /* Workspace of q6_dense_linear_grad; `outputs` holds Q6_GRAD_* of what is asked
    for, `has_gate` whether gate is given, pack as above. */

@@ -85,12 +85,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "q6_qk_rmsnorm_rope_bf16": (_I, [_P, _I64, _I64, _I, _I, _P, _P, _P, _F, _P]),
     "q6_qk_rmsnorm_rope_joint_bf16": (_I, [_P, _I64, _I64, _I, _I, _P, _P, _P, _P, _I64, _I64, _I64, _F, _P]),
     "q6_dense_linear": (
-        _I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _SZ, _P],
+        _I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _I, _I, _P, _SZ, _P],
     ),
     "q6_dense_linear_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "q6_dense_linear_grad": (
         _I,
-        [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _SZ, _P],
+        [_P, _I64, _P, _I64, _P, _I64, _P, _I, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _SZ, _P],
     ),
     "q6_dense_linear_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I, _I, _I, _I]),
     "q6_layer_norm": (_I, [_P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _F, _I, _I, _I, _P]),

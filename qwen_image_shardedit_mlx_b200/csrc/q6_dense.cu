@@ -54,7 +54,7 @@ int launch_pack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t ro
 struct DzParams {
     const void* dy;
     int64_t ldy;
-    const void* z;  // [M, N] dense, or null
+    const void* z;  // [M, N] dense, element type Z of the kernel, or null
     const void* gate;
     int64_t ldg;
     void* dz;  // row stride ldz, or null
@@ -71,7 +71,7 @@ struct DzParams {
 // A block takes 32 * V columns and one strip of rows (all of one gate vector):
 // 32 column lanes x 8 row lanes.  V = 8: 16-byte accesses (N, strides and
 // addresses aligned); V = 1: any layout.
-template <typename T, int V>
+template <typename T, typename Z, int V>
 __global__ void __launch_bounds__(256) dz_kernel(DzParams p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -92,12 +92,16 @@ __global__ void __launch_bounds__(256) dz_kernel(DzParams p) {
     struct alignas(sizeof(T) * V) Group {
         T v[V];
     };
+    struct alignas(V == 8 ? 16 : sizeof(Z)) GroupZ {
+        Z v[V];
+    };
     if (in) {
 #pragma unroll 2
         for (; r < r_end; r += 8) {
             const Group gy = *reinterpret_cast<const Group*>(static_cast<const T*>(p.dy) + r * p.ldy + c0);
-            Group gz, out;
-            if (p.z) gz = *reinterpret_cast<const Group*>(static_cast<const T*>(p.z) + r * p.N + c0);
+            Group out;
+            GroupZ gz;
+            if (p.z) gz = *reinterpret_cast<const GroupZ*>(static_cast<const Z*>(p.z) + r * p.N + c0);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float dy = to_f(gy.v[i]);
@@ -160,7 +164,7 @@ void plan_strips(int64_t M, int64_t N, int64_t rows_per_gate, int64_t* strip_row
     *strips_per_gate = (rows_per_gate + rows - 1) / rows;
 }
 
-template <typename T>
+template <typename T, typename Z>
 int run_dz(DzParams p, int64_t M, void* dbias, void* dgate, cudaStream_t stream) {
     const int64_t gates = M / p.rows_per_gate, strips = gates * p.strips_per_gate;
     const bool vec = p.N % 8 == 0 && p.ldy % 8 == 0 && (!p.gate || p.ldg % 8 == 0) && aligned16(p.dy) &&
@@ -170,8 +174,8 @@ int run_dz(DzParams p, int64_t M, void* dbias, void* dgate, cudaStream_t stream)
     const int64_t sum_blocks = (p.N + 127) / 128;
     if (strips * p.col_blocks > kMaxGrid || gates * sum_blocks > kMaxGrid) return Q6_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(strips * p.col_blocks));
-    const cudaError_t e = vec ? launch_pdl(dz_kernel<T, 8>, grid, dim3(256), 0, stream, p)
-                              : launch_pdl(dz_kernel<T, 1>, grid, dim3(256), 0, stream, p);
+    const cudaError_t e = vec ? launch_pdl(dz_kernel<T, Z, 8>, grid, dim3(256), 0, stream, p)
+                              : launch_pdl(dz_kernel<T, Z, 1>, grid, dim3(256), 0, stream, p);
     if (e != cudaSuccess) return Q6_ERR_CUDA;
     if (dbias && launch_pdl(sum_strips_kernel<T>, dim3(static_cast<unsigned>(sum_blocks)), dim3(128), 0, stream,
                             static_cast<const float*>(p.db_part), strips, p.N, static_cast<T*>(dbias)) != cudaSuccess)
@@ -194,13 +198,12 @@ bool needs_pack(const void* p, int64_t ld) { return !aligned16(p) || ld % 8 != 0
 // Hands out 256-byte aligned parts of the caller's workspace.
 struct Carver {
     char* base;
-    size_t size, used = 0;
+    size_t used = 0;
     void* take(size_t bytes) {
         const size_t at = used;
         used += round_up(bytes);
         return base ? base + at : nullptr;
     }
-    bool fits() const { return used <= size; }
 };
 
 size_t forward_bytes(int64_t M, int64_t N, int64_t K, int pack) {
@@ -265,22 +268,26 @@ size_t q6_dense_linear_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int
 
 int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* gate,
                     int64_t ldg, int64_t rows_per_gate, const void* residual, int64_t ldr, void* y, void* preact,
-                    int64_t M, int64_t N, int64_t K, int dtype, int activation, void* workspace,
+                    int preact_dtype, int64_t M, int64_t N, int64_t K, int dtype, int activation, void* workspace,
                     size_t workspace_bytes, q6_stream_t stream_) {
     using namespace q6;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     const int st = check_common(M, N, K, dtype, activation, gate, ldg, rows_per_gate);
     if (st != Q6_OK) return st;
     if (!x || !w || !y) return Q6_ERR_INVALID_ARGUMENT;
+    if (preact && preact_dtype != dtype && preact_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
     if (!stride_ok(ldx, K, M) || !stride_ok(ldw, K, N) || (residual && !stride_ok(ldr, N, M)))
         return Q6_ERR_INVALID_ARGUMENT;
     for (const void* t : {x, w, bias, gate, residual, static_cast<const void*>(y), static_cast<const void*>(preact)})
         if (!element_aligned(t)) return Q6_ERR_ALIGNMENT;
+    if (preact && preact_dtype == Q6_DTYPE_F32 && reinterpret_cast<uintptr_t>(preact) % 4) return Q6_ERR_ALIGNMENT;
+    if (M == 1) ldx = pad8(K);  // a single row has no stride
+    if (N == 1) ldw = pad8(K);
     const int pack = (needs_pack(x, ldx) ? Q6_PACK_X : 0) | (needs_pack(w, ldw) ? Q6_PACK_W : 0);
     if (workspace && reinterpret_cast<uintptr_t>(workspace) % kAlign) return Q6_ERR_ALIGNMENT;
     const size_t need = forward_bytes(M, N, K, pack);
     if (need > (workspace ? workspace_bytes : 0)) return Q6_ERR_WORKSPACE;
-    Carver ws{static_cast<char*>(workspace), workspace_bytes};
+    Carver ws{static_cast<char*>(workspace)};
     DenseProduct a{};
     a.workspace_bytes = dense_product_workspace_bytes(M, N, K, false, false);
     a.workspace = ws.take(a.workspace_bytes);
@@ -314,20 +321,22 @@ int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     a.epi.residual = residual;
     a.epi.ldr = ldr;
     a.epi.preact = preact;
+    a.epi.preact_f32 = preact_dtype == Q6_DTYPE_F32;
     a.epi.activation = activation;
     return launch_dense_product(a, stream);
 }
 
 int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                         const void* preact, const void* gate, int64_t ldg, int64_t rows_per_gate, void* dx, void* dw,
-                         void* dbias, void* dgate, int64_t M, int64_t N, int64_t K, int dtype, int activation,
-                         void* workspace, size_t workspace_bytes, q6_stream_t stream_) {
+                         const void* preact, int preact_dtype, const void* gate, int64_t ldg, int64_t rows_per_gate,
+                         void* dx, void* dw, void* dbias, void* dgate, int64_t M, int64_t N, int64_t K, int dtype,
+                         int activation, void* workspace, size_t workspace_bytes, q6_stream_t stream_) {
     using namespace q6;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     const int st = check_common(M, N, K, dtype, activation, gate, ldg, rows_per_gate);
     if (st != Q6_OK) return st;
     if (!dy || (dw && !x) || (dx && !w)) return Q6_ERR_INVALID_ARGUMENT;
     if (!preact && (activation != Q6_ACT_NONE || dgate)) return Q6_ERR_INVALID_ARGUMENT;
+    if (preact && preact_dtype != dtype && preact_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
     if (dgate && !gate) return Q6_ERR_INVALID_ARGUMENT;
     if (!stride_ok(ldy, N, M) || (dw && !stride_ok(ldx, K, M)) || (dx && !stride_ok(ldw, K, N)))
         return Q6_ERR_INVALID_ARGUMENT;
@@ -337,12 +346,15 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
     const int outputs = (dx ? Q6_GRAD_X : 0) | (dw ? Q6_GRAD_W : 0) | (dbias ? Q6_GRAD_BIAS : 0) |
                         (dgate ? Q6_GRAD_GATE : 0);
     if (outputs == 0) return Q6_OK;
+    if (preact && preact_dtype == Q6_DTYPE_F32 && reinterpret_cast<uintptr_t>(preact) % 4) return Q6_ERR_ALIGNMENT;
+    if (M == 1) ldx = pad8(K), ldy = pad8(N);  // a single row has no stride
+    if (N == 1) ldw = pad8(K);
     const int pack = (needs_pack(x, ldx) ? Q6_PACK_X : 0) | (needs_pack(w, ldw) ? Q6_PACK_W : 0) |
                      (needs_pack(dy, ldy) ? Q6_PACK_DY : 0);
     if (workspace && reinterpret_cast<uintptr_t>(workspace) % kAlign) return Q6_ERR_ALIGNMENT;
     const size_t need = grad_bytes(M, N, K, rows_per_gate, activation, gate != nullptr, outputs, pack);
     if (need > (workspace ? workspace_bytes : 0)) return Q6_ERR_WORKSPACE;
-    Carver ws{static_cast<char*>(workspace), workspace_bytes};
+    Carver ws{static_cast<char*>(workspace)};
     const size_t product_bytes = product_bytes_grad(M, N, K, outputs);
     void* product_ws = ws.take(product_bytes);
 
@@ -365,8 +377,11 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
     if (dbias) z.db_part = static_cast<float*>(ws.take(part));
     if (dgate) z.dg_part = static_cast<float*>(ws.take(part));
     if (wants_dz || dbias || dgate) {
-        const int e = dtype == Q6_DTYPE_BF16 ? run_dz<__nv_bfloat16>(z, M, dbias, dgate, stream)
-                                             : run_dz<__half>(z, M, dbias, dgate, stream);
+        const bool f32 = z.z && preact_dtype == Q6_DTYPE_F32;
+        const int e = dtype == Q6_DTYPE_BF16 ? (f32 ? run_dz<__nv_bfloat16, float>(z, M, dbias, dgate, stream)
+                                                    : run_dz<__nv_bfloat16, __nv_bfloat16>(z, M, dbias, dgate, stream))
+                                             : (f32 ? run_dz<__half, float>(z, M, dbias, dgate, stream)
+                                                    : run_dz<__half, __half>(z, M, dbias, dgate, stream));
         if (e != Q6_OK) return e;
     }
     const void* t = wants_dz ? z.dz : dy;

@@ -118,5 +118,6 @@ int error_word_tc(bool clear);
 int error_word_gemv(bool clear);
 int error_word_skinny(bool clear);
 int error_word_sp(bool clear);
+int error_word_dense(bool clear);
 
 }  // namespace q6

@@ -149,7 +149,9 @@ def _linear_forward(x, weight, bias, activation, residual, gate, save_preact):
     shape = x.shape[:-1] + (n,)
     with _on(dev) as here:
         y = torch.empty(shape, dtype=x.dtype, device=dev)
-        z = torch.empty(shape, dtype=x.dtype, device=dev) if save_preact else None
+        # the gate's gradient sums act(z) itself: rounded to 16 bits, z would cost it as much as its own rounding
+        zdt = x.dtype if gate is None else torch.float32
+        z = torch.empty(shape, dtype=zdt, device=dev) if save_preact else None
         m = x.numel() // k
         if m == 0:
             return y, z
@@ -165,7 +167,7 @@ def _linear_forward(x, weight, bias, activation, residual, gate, save_preact):
         ws = _workspace(nbytes, dev)
         _lib.check(
             lib.q6_dense_linear(xp, ldx, wp, ldw, _ptr(b2), _ptr(g2), ldg, rows_per_gate, _ptr(r2), ldr,
-                                y.data_ptr(), _ptr(z), m, n, k, _DTYPES[x.dtype], ACTIVATIONS[activation], _ptr(ws),
+                                y.data_ptr(), _ptr(z), _DTYPES[zdt], m, n, k, _DTYPES[x.dtype], ACTIVATIONS[activation], _ptr(ws),
                                 nbytes, here.stream), "q6_dense_linear")
     return y, z
 
@@ -181,8 +183,8 @@ def dense_linear_forward(
     save_preact: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(y, preact): ``dense_linear`` without autograd.  With ``save_preact`` the
-    second value is ``x @ W^T + bias`` rounded to x's dtype, which
-    ``dense_linear_backward`` takes; else None."""
+    second value is ``x @ W^T + bias`` (in x's dtype, or in fp32 when a gate is
+    given), which ``dense_linear_backward`` takes; else None."""
 
     with torch.no_grad():
         return _linear_forward(x, weight, bias, activation, residual, gate, save_preact)
@@ -229,7 +231,7 @@ def dense_linear_backward(
     if preact is not None and preact.shape != dy.shape:
         raise ValueError(f"preact must be {tuple(dy.shape)}, got {tuple(preact.shape)}")
     for name, t in (("x", x), ("weight", weight), ("preact", preact), ("gate", gate)):
-        if t is not None and t.dtype != dy.dtype:
+        if t is not None and t.dtype != dy.dtype and not (t is preact and t.dtype == torch.float32):
             raise ValueError(f"{name} is {t.dtype}, dy is {dy.dtype}")
     m = dy.numel() // n
     rows_per_gate = m if gate is None else _sample_rows("gate", gate, dy, n)
@@ -258,7 +260,8 @@ def dense_linear_backward(
         nbytes = lib.q6_dense_linear_grad_workspace_bytes(m, n, k, rows_per_gate, act, int(gate is not None), bits, pack)
         ws = _workspace(nbytes, dev)
         _lib.check(
-            lib.q6_dense_linear_grad(dyp, ldy, xp, ldx, wp, ldw, _ptr(z2), _ptr(g2), ldg, rows_per_gate, _ptr(dx),
+            lib.q6_dense_linear_grad(dyp, ldy, xp, ldx, wp, ldw, _ptr(z2),
+                                     _DTYPES[dy.dtype if z2 is None else z2.dtype], _ptr(g2), ldg, rows_per_gate, _ptr(dx),
                                      _ptr(dw), _ptr(db), _ptr(dg), m, n, k, _DTYPES[dy.dtype], act, _ptr(ws), nbytes,
                                      here.stream), "q6_dense_linear_grad")
     return DenseGrads(dx, dw, db, dg)

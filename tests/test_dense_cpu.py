@@ -96,7 +96,7 @@ def test_c_entries_refuse_before_the_device():
 
     def linear(**kw):
         a = dict(x=256, ldx=64, w=256, ldw=64, bias=None, gate=None, ldg=0, rpg=4, res=None, ldr=0, y=256, pre=None,
-                 M=4, N=32, K=64, dtype=0, act=0, ws=None, wsb=0, stream=None) | kw
+                 pdt=0, M=4, N=32, K=64, dtype=0, act=0, ws=None, wsb=0, stream=None) | kw
         return lib.q6_dense_linear(*a.values())
 
     assert linear(x=None) == inv and linear(w=None) == inv and linear(y=None) == inv
@@ -104,14 +104,14 @@ def test_c_entries_refuse_before_the_device():
     assert linear(ldx=63) == inv and linear(ldw=60) == inv and linear(res=256, ldr=31) == inv
     assert linear(rpg=3) == inv and linear(rpg=0) == inv and linear(rpg=2, gate=256, ldg=16) == inv
     assert linear(act=3) == inv and linear(act=-1) == inv
-    assert linear(dtype=2) == uns
+    assert linear(dtype=2) == uns and linear(pre=256, pdt=1) == uns and linear(pre=258, pdt=2) == al
     assert linear(x=257) == al and linear(y=255) == al and linear(ws=128, wsb=1 << 30) == al
     assert linear(x=258) == wsp  # an operand off its 16 bytes is copied: the workspace must hold it
     assert lib.q6_dense_linear_workspace_bytes(4, 32, 64, _lib.Q6_PACK_X) >= 4 * 64 * 2
     assert lib.q6_dense_linear_workspace_bytes(0, 32, 64, 0) == 0
 
     def grad(**kw):
-        a = dict(dy=256, ldy=32, x=256, ldx=64, w=256, ldw=64, pre=None, gate=None, ldg=0, rpg=4, dx=256, dw=256,
+        a = dict(dy=256, ldy=32, x=256, ldx=64, w=256, ldw=64, pre=None, pdt=1, gate=None, ldg=0, rpg=4, dx=256, dw=256,
                  db=256, dg=None, M=4, N=32, K=64, dtype=1, act=0, ws=None, wsb=0, stream=None) | kw
         return lib.q6_dense_linear_grad(*a.values())
 

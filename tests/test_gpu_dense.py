@@ -69,7 +69,8 @@ def check_linear(x, w, b, g, r, dy, activation, *, strict=True):
     ry, rz = bounds.linear(bx, bw, bb, activation, bg, br, dtype)
     ry.check(rows_of(y, n), "y")
     bdy = B(rows_of(dy, n))
-    dx, dw, db, dg = bounds.linear_grads(bdy, bx, bw, rz.round(dtype), activation, bg, dtype, groups)
+    dx, dw, db, dg = bounds.linear_grads(bdy, bx, bw, rz.round(dtype if g is None else torch.float32), activation, bg,
+                                          dtype, groups)
     dx.check(rows_of(grads["x"], k), "dx")
     dw.check(grads["w"], "dw")
     if b is not None:
@@ -469,7 +470,7 @@ def test_feed_forward_half_forward_and_backward(dtype):
     ra, z1 = bounds.linear(rh, bw1, bb1, "gelu_tanh", None, None, dtype)
     ry, z2 = bounds.linear(ra, bw2, bb2, None, bg, bx, dtype)
     ry.check(rows_of(y.detach(), d), "y")
-    da, dw2, db2, dgate = bounds.linear_grads(bdy, ra, bw2, z2.round(dtype), None, bg, dtype, s)
+    da, dw2, db2, dgate = bounds.linear_grads(bdy, ra, bw2, z2.round(torch.float32), None, bg, dtype, s)
     dh, dw1, db1, _ = bounds.linear_grads(da, rh, bw1, z1.round(dtype), "gelu_tanh", None, dtype, s)
     dxn, dscale, dshift = bounds.norm_grads(dh, xh, rstd, one, dtype, dtype, s)
     dx = (dxn + bdy).round(dtype)
