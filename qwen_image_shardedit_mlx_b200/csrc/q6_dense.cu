@@ -29,25 +29,66 @@ int64_t pad8(int64_t v) { return (v + 7) / 8 * 8; }
 
 // ------------------------------------------------------------------- aligned copy
 
-// dst [rows, cols] with row stride ldd from src with row stride lds, 16-bit
-// elements; the pad columns of dst are left alone (the tensor maps end at cols).
-__global__ void __launch_bounds__(256) pack_rows_kernel(const uint16_t* __restrict__ src, int64_t lds, uint16_t* dst,
-                                                        int64_t ldd, int64_t rows, int64_t cols) {
+// Up to two operands [rows, cols] copied to row stride ldd, 16-bit elements; the
+// pad columns are left alone (the tensor maps end at cols).  A block copies
+// 2048 neighbouring columns of kPackRows rows, eight columns per thread and one
+// 16-byte store for them.
+struct PackOne {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t lds, ldd, rows, cols;
+    unsigned col_blocks, blocks;
+};
+constexpr int kPackRows = 4;
+
+__global__ void __launch_bounds__(256) pack_rows_kernel(const PackOne first, const PackOne second) {
     pdl_launch_dependents();
     pdl_wait();
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
-        for (int64_t c = blockIdx.x * int64_t(256) + threadIdx.x; c < cols; c += int64_t(gridDim.x) * 256)
-            dst[r * ldd + c] = src[r * lds + c];
+    const bool one = blockIdx.x < first.blocks;
+    const PackOne p = one ? first : second;
+    const unsigned block = one ? blockIdx.x : blockIdx.x - first.blocks;
+    const int64_t c0 = block % p.col_blocks * int64_t(2048) + threadIdx.x * 8;
+    const int64_t r0 = block / p.col_blocks * int64_t(kPackRows);
+    if (c0 >= p.cols) return;
+    uint16_t v[kPackRows][8];
+#pragma unroll
+    for (int k = 0; k < kPackRows; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[k][i] = r0 + k < p.rows && c0 + i < p.cols ? __ldg(p.src + (r0 + k) * p.lds + c0 + i) : uint16_t(0);
+#pragma unroll
+    for (int k = 0; k < kPackRows; ++k)
+        if (r0 + k < p.rows)
+            *reinterpret_cast<uint4*>(p.dst + (r0 + k) * p.ldd + c0) =
+                make_uint4(v[k][0] | uint32_t(v[k][1]) << 16, v[k][2] | uint32_t(v[k][3]) << 16,
+                           v[k][4] | uint32_t(v[k][5]) << 16, v[k][6] | uint32_t(v[k][7]) << 16);
 }
 
-int launch_pack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t stream) {
-    const unsigned gx = static_cast<unsigned>(std::min<int64_t>((cols + 255) / 256, 1024));
-    const unsigned gy = static_cast<unsigned>(std::min<int64_t>(rows, std::max<int64_t>(1, 148 * 32 / gx)));
-    return launch_pdl(pack_rows_kernel, dim3(gx, gy), dim3(256), 0, stream, static_cast<const uint16_t*>(src), lds,
-                      static_cast<uint16_t*>(dst), ldd, rows, cols) == cudaSuccess
-               ? Q6_OK
-               : Q6_ERR_CUDA;
-}
+// The operands of one call that need an aligned copy (at most two).
+struct Packer {
+    PackOne part[2] = {};
+    int n = 0;
+    void add(const void* src, int64_t lds, void* dst, int64_t rows, int64_t cols) {
+        PackOne& p = part[n++];
+        p.src = static_cast<const uint16_t*>(src);
+        p.dst = static_cast<uint16_t*>(dst);
+        p.lds = lds;
+        p.ldd = pad8(cols);
+        p.rows = rows;
+        p.cols = cols;
+        p.col_blocks = static_cast<unsigned>((cols + 2047) / 2048);
+        p.blocks = static_cast<unsigned>(std::min<int64_t>(p.col_blocks * ((rows + kPackRows - 1) / kPackRows), kMaxGrid));
+    }
+    int launch(cudaStream_t stream) const {
+        if (n == 0) return Q6_OK;
+        const int64_t blocks = int64_t(part[0].blocks) + part[1].blocks;
+        if (blocks > kMaxGrid) return Q6_ERR_UNSUPPORTED;
+        return launch_pdl(pack_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, part[0],
+                          part[1]) == cudaSuccess
+                   ? Q6_OK
+                   : Q6_ERR_CUDA;
+    }
+};
 
 // ---------------------------------------------------------- elementwise backward
 
@@ -65,126 +106,144 @@ struct DzParams {
     int64_t rows_per_gate;
     int64_t strip_rows, strips_per_gate;
     unsigned col_blocks;
-    int activation;
 };
 
-// A block takes 32 * V columns and one strip of rows (all of one gate vector):
-// 32 column lanes x 8 row lanes.  V = 8: 16-byte accesses (N, strides and
-// addresses aligned); V = 1: any layout.
-template <typename T, typename Z, int V>
+// A block takes 256 V neighbouring columns, V per thread, and one strip of rows
+// (all of one gate vector), kRows rows' loads in flight at a time.  V = 8:
+// 16-byte accesses (N, strides and addresses aligned); V = 1: any layout.
+template <typename T, typename Z, int V, int ACT>
 __global__ void __launch_bounds__(256) dz_kernel(DzParams p) {
+    constexpr int kRows = 4;
     pdl_launch_dependents();
     pdl_wait();
-    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const int64_t col_block = blockIdx.x % p.col_blocks, strip = blockIdx.x / p.col_blocks;
-    const int64_t c0 = (col_block * 32 + cl) * V;
+    const int64_t c0 = (col_block * 256 + threadIdx.x) * V;
+    if (c0 >= p.N) return;
     const int64_t s = strip / p.strips_per_gate;
-    const int64_t r_end = std::min((s + 1) * p.rows_per_gate,
-                                   s * p.rows_per_gate + (strip % p.strips_per_gate + 1) * p.strip_rows);
-    int64_t r = s * p.rows_per_gate + (strip % p.strips_per_gate) * p.strip_rows + rl;
-    const bool in = c0 < p.N;
-    float gate[V], db[V], dg[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        gate[i] = in && p.gate ? to_f(static_cast<const T*>(p.gate)[s * p.ldg + c0 + i]) : 1.0f;
-        db[i] = dg[i] = 0.0f;
-    }
+    const int64_t r_begin = s * p.rows_per_gate + strip % p.strips_per_gate * p.strip_rows;
+    const int64_t r_end = min(r_begin + p.strip_rows, (s + 1) * p.rows_per_gate);
     struct alignas(sizeof(T) * V) Group {
         T v[V];
     };
     struct alignas(V == 8 ? 16 : sizeof(Z)) GroupZ {
         Z v[V];
     };
-    if (in) {
-#pragma unroll 2
-        for (; r < r_end; r += 8) {
-            const Group gy = *reinterpret_cast<const Group*>(static_cast<const T*>(p.dy) + r * p.ldy + c0);
-            Group out;
-            GroupZ gz;
-            if (p.z) gz = *reinterpret_cast<const GroupZ*>(static_cast<const Z*>(p.z) + r * p.N + c0);
+    const T* dyp = static_cast<const T*>(p.dy) + c0;
+    const Z* zp = static_cast<const Z*>(p.z) + c0;
+    Group gate{};
+    if (p.gate) gate = load_ro<Group>(static_cast<const T*>(p.gate) + s * p.ldg + c0);
+    float db[V], dg[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float dy = to_f(gy.v[i]);
-                float a = 0.0f, slope = 1.0f;
-                if (p.z) act_and_slope_f(to_f(gz.v[i]), p.activation, a, slope);
-                const float dz = dy * gate[i] * slope;
-                db[i] += dz;
-                dg[i] = fmaf(dy, a, dg[i]);
-                out.v[i] = from_f<T>(dz);
+    for (int i = 0; i < V; ++i) db[i] = dg[i] = 0.0f;
+    for (int64_t r0 = r_begin; r0 < r_end; r0 += kRows) {
+        Group gy[kRows];
+        GroupZ gz[kRows];
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t r = min(r0 + k, r_end - 1);
+            gy[k] = load_ro<Group>(dyp + r * p.ldy);
+            if (p.z) gz[k] = load_ro<GroupZ>(zp + r * p.N);
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            if (r0 + k < r_end) {
+                Group out;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float dy = to_f(gy[k].v[i]);
+                    float a = 0.0f, slope = 1.0f;
+                    if (p.z) act_and_slope_f(to_f(gz[k].v[i]), ACT, a, slope);
+                    const float dz = (p.gate ? dy * to_f(gate.v[i]) : dy) * slope;
+                    db[i] += dz;
+                    dg[i] = fmaf(dy, a, dg[i]);
+                    out.v[i] = from_f<T>(dz);
+                }
+                if (p.dz) *reinterpret_cast<Group*>(static_cast<T*>(p.dz) + (r0 + k) * p.ldz + c0) = out;
             }
-            if (p.dz) *reinterpret_cast<Group*>(static_cast<T*>(p.dz) + r * p.ldz + c0) = out;
         }
     }
-    // column sums over the eight row lanes, in order
-    __shared__ float sum[8][32 * V];
-    for (int pass = 0; pass < 2; ++pass) {
-        float* part = pass == 0 ? p.db_part : p.dg_part;
-        if (!part) continue;  // the same for the whole block
-        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[rl][cl * V + i] = pass == 0 ? db[i] : dg[i];
-        __syncthreads();
-        for (int c = threadIdx.x; c < 32 * V; c += 256) {
-            const int64_t col = col_block * (32 * V) + c;
-            if (col < p.N) {
-                float t = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) t += sum[k][c];
-                part[strip * p.N + col] = t;
-            }
-        }
+    for (int i = 0; i < V; ++i) {
+        if (p.db_part) p.db_part[strip * p.N + c0 + i] = db[i];
+        if (p.dg_part) p.dg_part[strip * p.N + c0 + i] = dg[i];
     }
 }
 
-// out[g, n] = sum over group g's strips of part[strip, n], in order.
+// dbias[n] = sum over all strips, dgate[g, n] = sum over gate vector g's strips, of
+// the strips' partial sums, in order: 32 columns x 8 strip lanes per block.  The
+// first db_blocks blocks sum dbias (none without it), the others dgate.
 template <typename T>
-__global__ void __launch_bounds__(128) sum_strips_kernel(const float* __restrict__ part, int64_t strips_per_group,
-                                                         int64_t N, T* out) {
+__global__ void __launch_bounds__(256) sum_strips_kernel(const float* db_part, const float* dg_part, int64_t strips,
+                                                         int64_t strips_per_gate, int64_t N, unsigned db_blocks,
+                                                         T* dbias, T* dgate) {
+    __shared__ float sum[8][33];
     pdl_launch_dependents();
     pdl_wait();
-    const unsigned col_blocks = static_cast<unsigned>((N + 127) / 128);
-    const int64_t n = blockIdx.x % col_blocks * int64_t(128) + threadIdx.x, group = blockIdx.x / col_blocks;
-    if (n >= N) return;
-    const float* src = part + group * strips_per_group * N + n;
+    const bool is_db = blockIdx.x < db_blocks;
+    const unsigned block = is_db ? blockIdx.x : blockIdx.x - db_blocks;
+    const unsigned col_blocks = static_cast<unsigned>((N + 31) / 32);
+    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
+    const int64_t n = block % col_blocks * int64_t(32) + cl, group = block / col_blocks;
+    const int64_t count = is_db ? strips : strips_per_gate;
+    const float* part = (is_db ? db_part : dg_part) + group * count * N;
     float t = 0.0f;
-#pragma unroll 8
-    for (int64_t i = 0; i < strips_per_group; ++i) t += src[i * N];
-    out[group * N + n] = from_f<T>(t);
+    if (n < N)
+        for (int64_t i = sl; i < count; i += 80) {
+            float f[10];
+#pragma unroll
+            for (int k = 0; k < 10; ++k) f[k] = i + 8 * k < count ? __ldcg(part + (i + 8 * k) * N + n) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 10; ++k) t += f[k];
+        }
+    sum[sl][cl] = t;
+    __syncthreads();
+    if (sl == 0 && n < N) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) t += sum[i][cl];
+        (is_db ? dbias : dgate)[group * N + n] = from_f<T>(t);
+    }
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// Rows per strip: enough blocks for the GPU, strips of 32 rows at least.
+// Rows per strip: about four blocks per SM, strips of 4 rows at least.  One plan
+// for both access widths (the narrow one only has more column blocks).
 void plan_strips(int64_t M, int64_t N, int64_t rows_per_gate, int64_t* strip_rows, int64_t* strips_per_gate) {
-    const int64_t col_blocks = (N + 255) / 256, gates = M / rows_per_gate;
-    const int64_t want = std::max<int64_t>(1, (148 * 4 + col_blocks * gates - 1) / (col_blocks * gates));
-    int64_t rows = std::max<int64_t>(32, (rows_per_gate + want - 1) / want);
-    rows = std::min(rows, rows_per_gate);
-    *strip_rows = rows;
-    *strips_per_gate = (rows_per_gate + rows - 1) / rows;
+    const int64_t blocks = (N + 2047) / 2048 * (M / rows_per_gate);
+    const int64_t want = std::max<int64_t>(1, (int64_t(device_sm_count()) * 4 + blocks - 1) / blocks);
+    *strip_rows = std::min(rows_per_gate, std::max<int64_t>(4, (rows_per_gate + want - 1) / want));
+    *strips_per_gate = (rows_per_gate + *strip_rows - 1) / *strip_rows;
 }
 
-template <typename T, typename Z>
+template <typename T, typename Z, int ACT>
 int run_dz(DzParams p, int64_t M, void* dbias, void* dgate, cudaStream_t stream) {
     const int64_t gates = M / p.rows_per_gate, strips = gates * p.strips_per_gate;
     const bool vec = p.N % 8 == 0 && p.ldy % 8 == 0 && (!p.gate || p.ldg % 8 == 0) && aligned16(p.dy) &&
                      aligned16(p.z) && aligned16(p.gate);
-    const int cols = vec ? 256 : 32;
+    const int cols = vec ? 2048 : 256;
     p.col_blocks = static_cast<unsigned>((p.N + cols - 1) / cols);
-    const int64_t sum_blocks = (p.N + 127) / 128;
-    if (strips * p.col_blocks > kMaxGrid || gates * sum_blocks > kMaxGrid) return Q6_ERR_UNSUPPORTED;
+    const int64_t db_blocks = dbias ? (p.N + 31) / 32 : 0, dg_blocks = dgate ? gates * ((p.N + 31) / 32) : 0;
+    if (strips * p.col_blocks > kMaxGrid || db_blocks + dg_blocks > kMaxGrid) return Q6_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(strips * p.col_blocks));
-    const cudaError_t e = vec ? launch_pdl(dz_kernel<T, Z, 8>, grid, dim3(256), 0, stream, p)
-                              : launch_pdl(dz_kernel<T, Z, 1>, grid, dim3(256), 0, stream, p);
+    const cudaError_t e = vec ? launch_pdl(dz_kernel<T, Z, 8, ACT>, grid, dim3(256), 0, stream, p)
+                              : launch_pdl(dz_kernel<T, Z, 1, ACT>, grid, dim3(256), 0, stream, p);
     if (e != cudaSuccess) return Q6_ERR_CUDA;
-    if (dbias && launch_pdl(sum_strips_kernel<T>, dim3(static_cast<unsigned>(sum_blocks)), dim3(128), 0, stream,
-                            static_cast<const float*>(p.db_part), strips, p.N, static_cast<T*>(dbias)) != cudaSuccess)
-        return Q6_ERR_CUDA;
-    if (dgate && launch_pdl(sum_strips_kernel<T>, dim3(static_cast<unsigned>(gates * sum_blocks)), dim3(128), 0, stream,
-                            static_cast<const float*>(p.dg_part), p.strips_per_gate, p.N,
-                            static_cast<T*>(dgate)) != cudaSuccess)
-        return Q6_ERR_CUDA;
-    return Q6_OK;
+    if (db_blocks + dg_blocks == 0) return Q6_OK;
+    return launch_pdl(sum_strips_kernel<T>, dim3(static_cast<unsigned>(db_blocks + dg_blocks)), dim3(256), 0, stream,
+                      static_cast<const float*>(p.db_part), static_cast<const float*>(p.dg_part), strips,
+                      p.strips_per_gate, p.N, static_cast<unsigned>(db_blocks), static_cast<T*>(dbias),
+                      static_cast<T*>(dgate)) == cudaSuccess
+               ? Q6_OK
+               : Q6_ERR_CUDA;
+}
+
+template <typename T, typename Z>
+int run_dz_act(const DzParams& p, int activation, int64_t M, void* dbias, void* dgate, cudaStream_t stream) {
+    switch (activation) {
+        case Q6_ACT_GELU_TANH: return run_dz<T, Z, Q6_ACT_GELU_TANH>(p, M, dbias, dgate, stream);
+        case Q6_ACT_SILU: return run_dz<T, Z, Q6_ACT_SILU>(p, M, dbias, dgate, stream);
+        default: return run_dz<T, Z, Q6_ACT_NONE>(p, M, dbias, dgate, stream);
+    }
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
@@ -291,18 +350,20 @@ int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     DenseProduct a{};
     a.workspace_bytes = dense_product_workspace_bytes(M, N, K, false, false);
     a.workspace = ws.take(a.workspace_bytes);
+    Packer packer;
     if (pack & Q6_PACK_X) {
         void* c = ws.take(size_t(M) * pad8(K) * 2);
-        if (const int e = launch_pack(x, ldx, c, pad8(K), M, K, stream)) return e;
+        packer.add(x, ldx, c, M, K);
         x = c;
         ldx = pad8(K);
     }
     if (pack & Q6_PACK_W) {
         void* c = ws.take(size_t(N) * pad8(K) * 2);
-        if (const int e = launch_pack(w, ldw, c, pad8(K), N, K, stream)) return e;
+        packer.add(w, ldw, c, N, K);
         w = c;
         ldw = pad8(K);
     }
+    if (const int e = packer.launch(stream)) return e;
     a.p = w;
     a.ldp = ldw;
     a.p_t = false;
@@ -366,7 +427,6 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
     z.ldg = ldg;
     z.N = N;
     z.rows_per_gate = rows_per_gate;
-    z.activation = activation;
     plan_strips(M, N, rows_per_gate, &z.strip_rows, &z.strips_per_gate);
     const size_t part = size_t(M / rows_per_gate) * z.strips_per_gate * N * sizeof(float);
     const bool wants_dz = writes_dz(activation, gate != nullptr, outputs, pack);
@@ -378,21 +438,32 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
     if (dgate) z.dg_part = static_cast<float*>(ws.take(part));
     if (wants_dz || dbias || dgate) {
         const bool f32 = z.z && preact_dtype == Q6_DTYPE_F32;
-        const int e = dtype == Q6_DTYPE_BF16 ? (f32 ? run_dz<__nv_bfloat16, float>(z, M, dbias, dgate, stream)
-                                                    : run_dz<__nv_bfloat16, __nv_bfloat16>(z, M, dbias, dgate, stream))
-                                             : (f32 ? run_dz<__half, float>(z, M, dbias, dgate, stream)
-                                                    : run_dz<__half, __half>(z, M, dbias, dgate, stream));
+        int e;
+        if (dtype == Q6_DTYPE_BF16)
+            e = f32 ? run_dz_act<__nv_bfloat16, float>(z, activation, M, dbias, dgate, stream)
+                    : run_dz_act<__nv_bfloat16, __nv_bfloat16>(z, activation, M, dbias, dgate, stream);
+        else
+            e = f32 ? run_dz_act<__half, float>(z, activation, M, dbias, dgate, stream)
+                    : run_dz_act<__half, __half>(z, activation, M, dbias, dgate, stream);
         if (e != Q6_OK) return e;
     }
     const void* t = wants_dz ? z.dz : dy;
     const int64_t ldt = wants_dz ? z.ldz : ldy;
+    Packer packer;
+    if (dx && (pack & Q6_PACK_W)) {
+        void* c = ws.take(size_t(N) * pad8(K) * 2);
+        packer.add(w, ldw, c, N, K);
+        w = c;
+        ldw = pad8(K);
+    }
+    if (dw && (pack & Q6_PACK_X)) {
+        void* c = ws.take(size_t(M) * pad8(K) * 2);
+        packer.add(x, ldx, c, M, K);
+        x = c;
+        ldx = pad8(K);
+    }
+    if (const int e = packer.launch(stream)) return e;
     if (dx) {
-        if (pack & Q6_PACK_W) {
-            void* c = ws.take(size_t(N) * pad8(K) * 2);
-            if (const int e = launch_pack(w, ldw, c, pad8(K), N, K, stream)) return e;
-            w = c;
-            ldw = pad8(K);
-        }
         DenseProduct a{};  // dx[m, k] = sum_n dz[m, n] W[n, k]
         a.p = w;
         a.ldp = ldw;
@@ -410,12 +481,6 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
         if (const int e = launch_dense_product(a, stream)) return e;
     }
     if (dw) {
-        if (pack & Q6_PACK_X) {
-            void* c = ws.take(size_t(M) * pad8(K) * 2);
-            if (const int e = launch_pack(x, ldx, c, pad8(K), M, K, stream)) return e;
-            x = c;
-            ldx = pad8(K);
-        }
         DenseProduct a{};  // dw[n, k] = sum_m dz[m, n] x[m, k]
         a.p = x;
         a.ldp = ldx;

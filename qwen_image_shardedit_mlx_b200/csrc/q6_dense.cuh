@@ -30,30 +30,67 @@ __device__ __forceinline__ float from_f<float>(float v) { return v; }
 constexpr float kGelu2K = 2.0f * 0.7978845608028654f;  // 2 sqrt(2 / pi)
 constexpr float kGeluC = 0.044715f;
 
-__device__ __forceinline__ float sigmoid_f(float s) { return __fdividef(1.0f, 1.0f + __expf(-s)); }
-
-__device__ __forceinline__ float act_f(float z, int act) {
-    if (act == Q6_ACT_GELU_TANH) return z * sigmoid_f(kGelu2K * z * fmaf(kGeluC * z, z, 1.0f));
-    if (act == Q6_ACT_SILU) return z * sigmoid_f(z);
-    return z;
+// 2^x and 1 / x by the hardware (relative errors near 2^-22); infinities give 0.
+__device__ __forceinline__ float ex2_f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_f(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// act(z) and act'(z) = s + z s (1 - s) ds/dz.  Beyond |z| = 12 the second term
-// is below 1e-30 for GELU; z is held there so that z^2 cannot overflow into 0 * inf.
-__device__ __forceinline__ void act_and_slope_f(float z, int act, float& a, float& slope) {
+constexpr float kLog2e = 1.4426950408889634f;
+
+// act(z) = z s, and s for the slope; t = z^2 is held at 400 (|z| = 20, where s is
+// 0 or 1 to the last bit), so that no product of infinities with zeros can arise.
+__device__ __forceinline__ float act_sigmoid(float z, int act, float& t) {
     if (act == Q6_ACT_GELU_TANH) {
-        const float s = sigmoid_f(kGelu2K * z * fmaf(kGeluC * z, z, 1.0f));
-        const float h = fminf(fmaxf(z, -12.0f), 12.0f);
-        a = z * s;
-        slope = fmaf(h * s * (1.0f - s), kGelu2K * fmaf(3.0f * kGeluC * h, h, 1.0f), s);
-    } else if (act == Q6_ACT_SILU) {
-        const float s = sigmoid_f(z);
-        a = z * s;
-        slope = fmaf(z * (1.0f - s), s, s);
-    } else {
+        t = fminf(z * z, 400.0f);
+        return rcp_f(1.0f + ex2_f(z * fmaf(t, -kLog2e * kGelu2K * kGeluC, -kLog2e * kGelu2K)));
+    }
+    return rcp_f(1.0f + ex2_f(-kLog2e * z));
+}
+
+__device__ __forceinline__ float act_f(float z, int act) {
+    if (act == Q6_ACT_NONE) return z;
+    float t;
+    return z * act_sigmoid(z, act, t);
+}
+
+// act(z) and act'(z) = s + z s (1 - s) du/dz, u the sigmoid's argument.
+__device__ __forceinline__ void act_and_slope_f(float z, int act, float& a, float& slope) {
+    if (act == Q6_ACT_NONE) {
         a = z;
         slope = 1.0f;
+        return;
     }
+    float t;
+    const float s = act_sigmoid(z, act, t);
+    a = z * s;
+    const float q = a * (1.0f - s);
+    slope = act == Q6_ACT_GELU_TANH ? fmaf(q, fmaf(t, 3.0f * kGelu2K * kGeluC, kGelu2K), s) : q + s;
+}
+
+// 16-byte (or smaller) read-only loads: free to move across stores.
+template <typename S>
+__device__ __forceinline__ S load_ro(const void* p) {
+    static_assert(sizeof(S) == 2 || sizeof(S) == 4 || sizeof(S) == 8 || sizeof(S) % 16 == 0, "load size");
+    S out;
+    if constexpr (sizeof(S) % 16 == 0) {
+        uint4* o = reinterpret_cast<uint4*>(&out);
+#pragma unroll
+        for (int i = 0; i < int(sizeof(S) / 16); ++i) o[i] = __ldg(static_cast<const uint4*>(p) + i);
+    } else if constexpr (sizeof(S) == 8) {
+        *reinterpret_cast<uint2*>(&out) = __ldg(static_cast<const uint2*>(p));
+    } else if constexpr (sizeof(S) == 4) {
+        *reinterpret_cast<uint32_t*>(&out) = __ldg(static_cast<const uint32_t*>(p));
+    } else {
+        *reinterpret_cast<uint16_t*>(&out) = __ldg(static_cast<const uint16_t*>(p));
+    }
+    return out;
 }
 
 }  // namespace q6

@@ -4,6 +4,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <cstdio>
 #include <cstdlib>
 #include <mutex>
 
@@ -51,9 +52,10 @@ __global__ void __launch_bounds__(256) dense_reduce_kernel(const DenseParams p) 
                 res = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(p.epi.residual) + r * p.epi.ldr + c);
             finish8<T>(p.epi, p.d, r, p.C, c, gate_row, bias, res, v);
         } else {
-            float v = 0.0f;
-            for (int s = 0; s < p.splits; ++s) v += src[s * plane];
-            finish1<T>(p.epi, p.d, r, p.C, c, gate_row, v);
+            float v[1] = {0.0f};
+            for (int s = 0; s < p.splits; ++s) v[0] += src[s * plane];
+            const float bias = p.epi.bias ? to_f(static_cast<const T*>(p.epi.bias)[c]) : 0.0f;
+            finish_column<T, 1>(p.epi, p.d, r, 1, p.C, c, p.gate_rows, bias, v);
         }
     }
 }
@@ -71,6 +73,15 @@ DensePlan plan_dense(int64_t R, int64_t C, int64_t L, bool q_t) {
         bool pair;
     };
     static const Shape kShapes[] = {{256, true}, {192, true}, {128, true}, {128, false}, {64, false}, {32, false}, {16, false}};
+    if (const char* v = std::getenv("Q6_DENSE_PLAN")) {  // "rows per tile,CTA pair,splits"
+        int ct = 0, pair = 0, splits = 0;
+        if (std::sscanf(v, "%d,%d,%d", &ct, &pair, &splits) == 3 && splits >= 1 && splits <= 16)
+            for (const Shape& sh : kShapes)
+                if (sh.ct == ct && sh.pair == (pair != 0) && !(q_t && (ct == 192 || ct < 64))) {
+                    const int64_t stages = ceil_div(L, dense_stage_depth(ct)), per = ceil_div(stages, splits);
+                    return DensePlan{ct, sh.pair, static_cast<int>(ceil_div(stages, per)), static_cast<int>(per)};
+                }
+    }
     DensePlan best{0, false, 1, 1};
     double best_cost = 0.0;
     for (const Shape& sh : kShapes) {

@@ -201,22 +201,36 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
     *reinterpret_cast<Eight<T>*>(static_cast<T*>(d) + at) = y;
 }
 
-// The same for one output of any layout.
-template <typename T>
-__device__ __forceinline__ void finish1(const DenseEpilogue& e, void* d, int64_t r, int64_t C, int c, int64_t gate_row,
-                                        float v) {
-    if (e.bias) v += to_f(static_cast<const T*>(e.bias)[c]);
-    const int64_t at = r * C + c;
-    if (e.preact) {
-        if (e.preact_f32)
-            static_cast<float*>(e.preact)[at] = v;
-        else
-            static_cast<T*>(e.preact)[at] = from_f<T>(v);
+// The same for kRows outputs of one column c (rows r .. r + n - 1 of them), any
+// layout; the rows' loads are issued together.
+template <typename T, int kRows>
+__device__ __forceinline__ void finish_column(const DenseEpilogue& e, void* d, int r, int n, int64_t C, int c,
+                                              int gate_rows, float bias, float (&v)[kRows]) {
+    T res[kRows], gate[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        if (i < n) {
+            if (e.residual) res[i] = static_cast<const T*>(e.residual)[(r + i) * e.ldr + c];
+            if (e.gate) gate[i] = static_cast<const T*>(e.gate)[(r + i) / gate_rows * e.ldg + c];
+        }
     }
-    v = act_f(v, e.activation);
-    if (e.gate) v *= to_f(static_cast<const T*>(e.gate)[gate_row * e.ldg + c]);
-    if (e.residual) v += to_f(static_cast<const T*>(e.residual)[r * e.ldr + c]);
-    static_cast<T*>(d)[at] = from_f<T>(v);
+    int64_t at = r * C + c;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i, at += C) {
+        if (i < n) {
+            float t = v[i] + bias;
+            if (e.preact) {
+                if (e.preact_f32)
+                    static_cast<float*>(e.preact)[at] = t;
+                else
+                    static_cast<T*>(e.preact)[at] = from_f<T>(t);
+            }
+            t = act_f(t, e.activation);
+            if (e.gate) t *= to_f(gate[i]);
+            if (e.residual) t += to_f(res[i]);
+            static_cast<T*>(d)[at] = from_f<T>(t);
+        }
+    }
 }
 
 // One warp's 32 columns (lanes of tensor memory) x kChunk rows.
@@ -268,12 +282,15 @@ __device__ __forceinline__ void dense_epilogue_block(const DenseParams& p, const
         }
     } else {
         const int c = c0 + lane;
-#pragma unroll 4
-        for (int j = 0; j < kChunk; ++j) {
-            const int r = r0 + j;
-            if (r < p.R && c < p.C)
-                finish1<T>(e, p.d, r, p.C, c, e.gate ? r / p.gate_rows : 0,
-                           stage[j * 32 + (lane ^ ((j & 1) << 2))]);
+        if (c < p.C) {
+            const float b = e.bias ? to_f(static_cast<const T*>(e.bias)[c]) : 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < kChunk && r0 + j < p.R; j += 8) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = stage[(j + i) * 32 + (lane ^ ((i & 1) << 2))];
+                finish_column<T, 8>(e, p.d, r0 + j, min(8, p.R - r0 - j), p.C, c, p.gate_rows, b, f);
+            }
         }
     }
     __syncwarp();

@@ -119,5 +119,6 @@ int error_word_gemv(bool clear);
 int error_word_skinny(bool clear);
 int error_word_sp(bool clear);
 int error_word_dense(bool clear);
+int error_word_norm(bool clear);
 
 }  // namespace q6

@@ -1,45 +1,34 @@
-// Layer norm over rows of D, forward and gradients (q6_layer_norm,
-// q6_layer_norm_grad):
-//   y = xh w + b,  xh = (x - mean) rstd
-//   a = dy w,  dx = rstd (a - mean_D(a) - xh mean_D(a xh)),
-//   dweight = sum over rows of dy xh,  dbias = sum over rows of dy.
-// Statistics and sums in fp32 (the variance from centred values, a second
-// pass); one rounding at each output.
-#include <algorithm>
-#include <cstdint>
-
-#include "q6_dense.cuh"
-#include "q6_internal.h"
-#include "q6_ptx.cuh"
+// Layer norm entry points (q6_layer_norm, q6_layer_norm_grad), the plain kernels
+// for rows wider than the register kernels hold (q6_norm.cuh), and the sums over
+// strips.
+#include "q6_norm.cuh"
 
 namespace q6 {
+
+void norm_plan_strips(int64_t M, int64_t rows_per_vec, int64_t least, int64_t* strip_rows, int64_t* strips_per_vec) {
+    const int64_t vecs = M / rows_per_vec, per = std::max<int64_t>(1, device_sm_count() / vecs);
+    *strip_rows = std::max<int64_t>(least, (rows_per_vec + per - 1) / per);
+    *strips_per_vec = (rows_per_vec + *strip_rows - 1) / *strip_rows;
+}
+
+#define Q6_NORM_DECLARE(T, V)                                                                                        \
+    template <>                                                                                                      \
+    int norm_forward_typed<T, V>(const NormParams& p, bool vec, int shape, cudaStream_t stream);                     \
+    template <>                                                                                                      \
+    int norm_grad_typed<T, V>(const NormParams& p, bool vec, int shape, V* dweight, V* dbias, cudaStream_t stream);
+Q6_NORM_DECLARE(__nv_bfloat16, __nv_bfloat16)
+Q6_NORM_DECLARE(__nv_bfloat16, float)
+Q6_NORM_DECLARE(__half, __half)
+Q6_NORM_DECLARE(__half, float)
+Q6_NORM_DECLARE(float, float)
+#undef Q6_NORM_DECLARE
+
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
 
-struct NormParams {
-    const void* x;
-    int64_t ldx;
-    const void* weight;
-    const void* bias;
-    int64_t ldv, rows_per_vec;
-    void* y;
-    float* mean;
-    float* rstd;
-    int64_t M, D;
-    float eps;
-    float one;  // added to the weight: 1 with Q6_NORM_ONE_PLUS
-    // gradients
-    const void* dy;
-    int64_t ldy;
-    void* dx;
-    float* dw_part;  // [strips, D] or null
-    float* db_part;
-    int64_t strip_rows, strips_per_vec;
-    unsigned col_blocks;
-};
-
+// Plain kernels for rows that do not fit the registers: any width, stride and
+// alignment.
 __device__ __forceinline__ float block_sum(float v) {
     __shared__ float part[kThreads / 32];
 #pragma unroll
@@ -108,8 +97,8 @@ __global__ void __launch_bounds__(kThreads) norm_rows_dx_kernel(NormParams p) {
 }
 
 // Partial column sums of dy xh and dy over one strip of rows.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_column_sums_kernel(NormParams p) {
+template <typename T, typename V>
+__global__ void __launch_bounds__(kThreads) norm_column_sums_kernel(NormParams p, V* dweight, V* dbias) {
     pdl_launch_dependents();
     pdl_wait();
     const int64_t strip = blockIdx.x / p.col_blocks;
@@ -126,66 +115,154 @@ __global__ void __launch_bounds__(kThreads) norm_column_sums_kernel(NormParams p
     }
     if (p.dw_part) p.dw_part[strip * p.D + c] = dw;
     if (p.db_part) p.db_part[strip * p.D + c] = db;
+    if (dweight) dweight[strip * p.D + c] = from_f<V>(dw);
+    if (dbias) dbias[strip * p.D + c] = from_f<V>(db);
 }
 
+// out[v, c] = sum over vector v's strips of part[strip, c], in order: 32
+// columns x 16 strip lanes per block, ten strips' loads in flight (a strip per
+// SM: one round trip).  The first half of the grid sums dweight, the second
+// dbias (either may be absent).
 template <typename V>
-__global__ void __launch_bounds__(128) norm_sum_strips_kernel(const float* __restrict__ part, int64_t strips_per_vec,
-                                                              int64_t D, V* out) {
+__global__ void __launch_bounds__(512) norm_sum_strips_kernel(const float* dw_part, const float* db_part,
+                                                              int64_t strips_per_vec, int64_t D, V* dweight,
+                                                              V* dbias) {
+    __shared__ float sum[16][33];
     pdl_launch_dependents();
+    const unsigned half = gridDim.x / 2;
+    const bool first = blockIdx.x < half;
+    const unsigned block = first ? blockIdx.x : blockIdx.x - half;
+    const float* part = first ? dw_part : db_part;
+    V* out = first ? dweight : dbias;
+    const unsigned col_blocks = static_cast<unsigned>((D + 31) / 32);
+    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
+    const int64_t c = block % col_blocks * int64_t(32) + cl, v = block / col_blocks;
     pdl_wait();
-    const unsigned col_blocks = static_cast<unsigned>((D + 127) / 128);
-    const int64_t c = blockIdx.x % col_blocks * int64_t(128) + threadIdx.x, v = blockIdx.x / col_blocks;
-    if (c >= D) return;
+    if (!part) return;
     float t = 0.0f;
-#pragma unroll 8
-    for (int64_t i = 0; i < strips_per_vec; ++i) t += part[(v * strips_per_vec + i) * D + c];
-    out[v * D + c] = from_f<V>(t);
+    if (c < D) {
+        const float* src = part + v * strips_per_vec * D + c;
+        for (int64_t i = sl; i < strips_per_vec; i += 160) {
+            float f[10];
+#pragma unroll
+            for (int k = 0; k < 10; ++k) f[k] = i + 16 * k < strips_per_vec ? __ldcg(src + (i + 16 * k) * D) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 10; ++k) t += f[k];
+        }
+    }
+    sum[sl][cl] = t;
+    __syncthreads();
+    if (sl == 0 && c < D) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) t += sum[i][cl];
+        out[v * D + c] = from_f<V>(t);
+    }
 }
 
-void plan_strips(int64_t M, int64_t rows_per_vec, int64_t* strip_rows, int64_t* strips_per_vec) {
-    const int64_t vecs = M / rows_per_vec, want = std::max<int64_t>(1, 592 / vecs);
-    *strip_rows = std::max<int64_t>(1, (rows_per_vec + want - 1) / want);
+// The plain kernels sum columns with one thread each: more, shorter strips.
+void plan_plain_strips(int64_t M, int64_t rows_per_vec, int64_t* strip_rows, int64_t* strips_per_vec) {
+    const int64_t vecs = M / rows_per_vec, per = std::max<int64_t>(1, 4 * device_sm_count() / vecs);
+    *strip_rows = (rows_per_vec + per - 1) / per;
     *strips_per_vec = (rows_per_vec + *strip_rows - 1) / *strip_rows;
 }
 
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
 
-size_t grad_bytes(int64_t M, int64_t D, int64_t rows_per_vec, int outputs) {
-    int64_t rows, per;
-    plan_strips(M, rows_per_vec, &rows, &per);
-    const size_t part = round_up(size_t(M / rows_per_vec) * per * D * sizeof(float));
+// The backward's shape for a row of D (an index into kNormGrad or, without 16-byte
+// accesses, kNormGradStrided; -1: the plain kernels) and its strips.
+int plan_grad(int64_t M, int64_t D, int64_t rows_per_vec, int dtype, bool vec, int64_t* strip_rows,
+              int64_t* strips_per_vec) {
+    const int shape = vec ? norm_shape(kNormGrad, D, dtype) : norm_shape(kNormGradStrided, D, dtype);
+    if (shape < 0)
+        plan_plain_strips(M, rows_per_vec, strip_rows, strips_per_vec);
+    else
+        norm_plan_strips(M, rows_per_vec,
+                         vec ? norm_detail::grad_row_lanes(kNormGrad[shape].w, kNormGrad[shape].n)
+                             : strided_row_lanes(kNormGradStrided[shape].w),
+                         strip_rows, strips_per_vec);
+    return shape;
+}
+
+// Bytes of one vector gradient's partial sums, for either access width (none where
+// a strip is a vector).
+size_t part_bytes(int64_t M, int64_t D, int64_t rows_per_vec, int dtype) {
+    int64_t rows, per, most = 1;
+    for (const bool vec : {true, false}) {
+        plan_grad(M, D, rows_per_vec, dtype, vec, &rows, &per);
+        most = std::max(most, per);
+    }
+    return most == 1 ? 0 : round_up(size_t(M / rows_per_vec) * most * D * sizeof(float));
+}
+
+size_t grad_bytes(int64_t M, int64_t D, int64_t rows_per_vec, int dtype, int outputs) {
+    const size_t part = part_bytes(M, D, rows_per_vec, dtype);
     return ((outputs & Q6_GRAD_W) ? part : 0) + ((outputs & Q6_GRAD_BIAS) ? part : 0);
 }
 
+bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// 16-byte accesses to every operand: G elements of T, and of V in 16-byte parts.
 template <typename T, typename V>
-int run_forward(const NormParams& p, cudaStream_t stream) {
+bool vector_ok(const NormParams& p) {
+    constexpr int64_t G = 16 / sizeof(T);
+    if (p.D % G || p.ldx % G || !al16(p.x) || !al16(p.weight) || !al16(p.bias)) return false;
+    if ((p.weight || p.bias) && p.rows_per_vec < p.M && p.ldv * sizeof(V) % 16) return false;
+    if (p.dy && (p.ldy % G || !al16(p.dy))) return false;
+    return al16(p.y) && al16(p.dx);
+}
+
+template <typename T, typename V>
+int run_forward(NormParams p, cudaStream_t stream) {
+    const int shape = norm_shape(kNormForward, p.D, sizeof(T) == 4 ? Q6_DTYPE_F32 : Q6_DTYPE_BF16);
+    if (shape >= 0) {
+        const int64_t vecs = p.M / p.rows_per_vec;
+        p.vecs = vecs > 1 && vecs <= 65535 ? static_cast<unsigned>(vecs) : 0;
+        return norm_forward_typed<T, V>(p, vector_ok<T, V>(p), shape, stream);
+    }
     return launch_pdl(norm_rows_kernel<T, V>, dim3(static_cast<unsigned>(p.M)), dim3(kThreads), 0, stream, p) ==
                    cudaSuccess
                ? Q6_OK
                : Q6_ERR_CUDA;
 }
 
+template <typename V>
+int sum_strips(const NormParams& p, void* dweight, void* dbias, cudaStream_t stream) {
+    const int64_t blocks = p.M / p.rows_per_vec * ((p.D + 31) / 32);
+    if (2 * blocks > kNormMaxGrid) return Q6_ERR_UNSUPPORTED;
+    return launch_pdl(norm_sum_strips_kernel<V>, dim3(static_cast<unsigned>(2 * blocks)), dim3(512), 0, stream,
+                      static_cast<const float*>(p.dw_part), static_cast<const float*>(p.db_part), p.strips_per_vec,
+                      p.D, static_cast<V*>(dweight), static_cast<V*>(dbias)) == cudaSuccess
+               ? Q6_OK
+               : Q6_ERR_CUDA;
+}
+
 template <typename T, typename V>
-int run_grad(const NormParams& p, void* dweight, void* dbias, cudaStream_t stream) {
+int run_grad(NormParams p, void* dweight, void* dbias, cudaStream_t stream) {
+    const bool vec = vector_ok<T, V>(p);
+    const int shape = plan_grad(p.M, p.D, p.rows_per_vec, sizeof(T) == 4 ? Q6_DTYPE_F32 : Q6_DTYPE_BF16, vec,
+                                &p.strip_rows, &p.strips_per_vec);
+    if (shape >= 0) {
+        if (p.M / p.rows_per_vec * p.strips_per_vec > kNormMaxGrid) return Q6_ERR_UNSUPPORTED;
+        const bool whole = p.strips_per_vec == 1;  // a strip is a vector: its sums are the result
+        if (whole) p.dw_part = p.db_part = nullptr;
+        const int st = norm_grad_typed<T, V>(p, vec, shape, whole ? static_cast<V*>(dweight) : static_cast<V*>(nullptr),
+                                             whole ? static_cast<V*>(dbias) : static_cast<V*>(nullptr), stream);
+        return st != Q6_OK || whole || (!dweight && !dbias) ? st : sum_strips<V>(p, dweight, dbias, stream);
+    }
     if (p.dx && launch_pdl(norm_rows_dx_kernel<T, V>, dim3(static_cast<unsigned>(p.M)), dim3(kThreads), 0, stream,
-                           p) != cudaSuccess)
+                           static_cast<const NormParams>(p)) != cudaSuccess)
         return Q6_ERR_CUDA;
     if (!dweight && !dbias) return Q6_OK;
-    const int64_t vecs = p.M / p.rows_per_vec, strips = vecs * p.strips_per_vec, sum_blocks = (p.D + 127) / 128;
-    if (strips * p.col_blocks > kMaxGrid || vecs * sum_blocks > kMaxGrid) return Q6_ERR_UNSUPPORTED;
-    if (launch_pdl(norm_column_sums_kernel<T>, dim3(static_cast<unsigned>(strips * p.col_blocks)), dim3(kThreads), 0,
-                   stream, p) != cudaSuccess)
+    const int64_t strips = p.M / p.rows_per_vec * p.strips_per_vec;
+    p.col_blocks = static_cast<unsigned>((p.D + kThreads - 1) / kThreads);
+    if (strips * p.col_blocks > kNormMaxGrid) return Q6_ERR_UNSUPPORTED;
+    const bool whole = p.strips_per_vec == 1;
+    if (whole) p.dw_part = p.db_part = nullptr;
+    if (launch_pdl(norm_column_sums_kernel<T, V>, dim3(static_cast<unsigned>(strips * p.col_blocks)), dim3(kThreads), 0,
+                   stream, static_cast<const NormParams>(p), whole ? static_cast<V*>(dweight) : static_cast<V*>(nullptr),
+                   whole ? static_cast<V*>(dbias) : static_cast<V*>(nullptr)) != cudaSuccess)
         return Q6_ERR_CUDA;
-    const dim3 grid(static_cast<unsigned>(vecs * sum_blocks));
-    if (dweight && launch_pdl(norm_sum_strips_kernel<V>, grid, dim3(128), 0, stream,
-                              static_cast<const float*>(p.dw_part), p.strips_per_vec, p.D,
-                              static_cast<V*>(dweight)) != cudaSuccess)
-        return Q6_ERR_CUDA;
-    if (dbias && launch_pdl(norm_sum_strips_kernel<V>, grid, dim3(128), 0, stream,
-                            static_cast<const float*>(p.db_part), p.strips_per_vec, p.D,
-                            static_cast<V*>(dbias)) != cudaSuccess)
-        return Q6_ERR_CUDA;
-    return Q6_OK;
+    return whole ? Q6_OK : sum_strips<V>(p, dweight, dbias, stream);
 }
 
 // Calls f with the element types of dtype / vec_dtype.
@@ -199,7 +276,7 @@ int with_types(int dtype, int vec_dtype, F&& f) {
 
 int check_norm(const void* x, int64_t ldx, int64_t ldv, int64_t rows_per_vec, int64_t M, int64_t D, int dtype,
                int vec_dtype, int flags, bool has_vec) {
-    if (!x || M <= 0 || D <= 0 || M > kMaxGrid || D > (int64_t(1) << 30)) return Q6_ERR_INVALID_ARGUMENT;
+    if (!x || M <= 0 || D <= 0 || M > kNormMaxGrid || D > (int64_t(1) << 30)) return Q6_ERR_INVALID_ARGUMENT;
     if (dtype < Q6_DTYPE_BF16 || dtype > Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
     if (vec_dtype != dtype && vec_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
     if (rows_per_vec <= 0 || rows_per_vec > M || M % rows_per_vec != 0) return Q6_ERR_INVALID_ARGUMENT;
@@ -214,6 +291,16 @@ bool aligned_to(const void* p, int dtype) {
 }
 
 }  // namespace
+
+int error_word_norm(bool clear) {
+    int code = 0;
+    for (const int w : {error_word_norm_bf16(clear), error_word_norm_f16(clear), error_word_norm_f32(clear)}) {
+        if (w < 0) return -1;
+        if (code == 0) code = w;
+    }
+    return code;
+}
+
 }  // namespace q6
 
 extern "C" {
@@ -248,9 +335,8 @@ int q6_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bi
 }
 
 size_t q6_layer_norm_grad_workspace_bytes(int64_t M, int64_t D, int64_t rows_per_vec, int dtype, int outputs) {
-    (void)dtype;
     if (M <= 0 || D <= 0 || rows_per_vec <= 0 || M % rows_per_vec != 0) return 0;
-    return q6::grad_bytes(M, D, rows_per_vec, outputs);
+    return q6::grad_bytes(M, D, rows_per_vec, dtype, outputs);
 }
 
 int q6_layer_norm_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* weight, int64_t ldv,
@@ -268,7 +354,7 @@ int q6_layer_norm_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, 
     const int outputs = (dweight ? Q6_GRAD_W : 0) | (dbias ? Q6_GRAD_BIAS : 0);
     if (!dx && !outputs) return Q6_OK;
     if (workspace && reinterpret_cast<uintptr_t>(workspace) % 256) return Q6_ERR_ALIGNMENT;
-    if (grad_bytes(M, D, rows_per_vec, outputs) > (workspace ? workspace_bytes : 0)) return Q6_ERR_WORKSPACE;
+    if (grad_bytes(M, D, rows_per_vec, dtype, outputs) > (workspace ? workspace_bytes : 0)) return Q6_ERR_WORKSPACE;
     NormParams p{};
     p.x = x;
     p.ldx = ldx;
@@ -283,9 +369,7 @@ int q6_layer_norm_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx, 
     p.dy = dy;
     p.ldy = ldy;
     p.dx = dx;
-    plan_strips(M, rows_per_vec, &p.strip_rows, &p.strips_per_vec);
-    p.col_blocks = static_cast<unsigned>((D + kThreads - 1) / kThreads);
-    const size_t part = round_up(size_t(M / rows_per_vec) * p.strips_per_vec * D * sizeof(float));
+    const size_t part = part_bytes(M, D, rows_per_vec, dtype);
     char* ws = static_cast<char*>(workspace);
     if (dweight) p.dw_part = reinterpret_cast<float*>(ws);
     if (dbias) p.db_part = reinterpret_cast<float*>(ws + (dweight ? part : 0));
