@@ -5,7 +5,9 @@
 Each .cu under csrc/ is compiled to an object under csrc/_build/ (skipped when
 up to date) and the objects are linked into qwen_image_shardedit_mlx_b200/libq6b200.so
 with a static CUDA runtime, so the library carries no dependency on a
-particular libcudart next to it.
+particular libcudart next to it.  The torch surface of the dense operators
+(csrc/q6_torch.cpp) becomes the extension module _q6torch next to it, linked
+against that library.
 """
 
 from __future__ import annotations
@@ -23,6 +25,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = CSRC / "_build"
 LIB = PKG / "libq6b200.so"
+EXT = PKG / "_q6torch.so"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -80,7 +83,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
             sys.stdout.write(res.stdout)
             sys.stderr.write(res.stderr)
         if res.returncode != 0:
-            raise RuntimeError(f"nvcc failed for {cmd[-3]}")
+            raise RuntimeError(f"{Path(cmd[0]).name} failed for {cmd[-3]}")
 
     if cmds:
         with ThreadPoolExecutor(max_workers=min(len(cmds), os.cpu_count() or 4)) as pool:
@@ -88,7 +91,27 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     if force or cmds or _needs(LIB, objs):
         link = [nvcc(), *ARCH, "-shared", "-cudart", "static", *[str(o) for o in objs], "-o", str(LIB)]
         run(link)
+    ext = CSRC / "q6_torch.cpp"
+    if force or _needs(EXT, [ext, INCLUDE / "q6_b200.h", LIB]):
+        run(_torch_extension_command(ext))
     return LIB
+
+
+def _torch_extension_command(src: Path) -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], str(INCLUDE)]
+    libs = cpp_extension.library_paths("cuda")
+    return [
+        shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        "-DTORCH_EXTENSION_NAME=_q6torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *[f"-I{p}" for p in includes], str(src), *[f"-L{p}" for p in [*libs, str(PKG)]],
+        "-l:libq6b200.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+        "-Wl,-rpath,$ORIGIN", "-o", str(EXT),
+    ]
 
 
 def main() -> int:
