@@ -13,6 +13,7 @@
 // equal calls give equal bits.
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 
 #include "q6_dense.cuh"
 #include "q6_dense.h"
@@ -108,64 +109,98 @@ struct DzParams {
     unsigned col_blocks;
 };
 
-// A block takes 256 V neighbouring columns, V per thread, and one strip of rows
-// (all of one gate vector), kRows rows' loads in flight at a time.  V = 8:
-// 16-byte accesses (N, strides and addresses aligned); V = 1: any layout.
-template <typename T, typename Z, int V, int ACT>
-__global__ void __launch_bounds__(256) dz_kernel(DzParams p) {
-    constexpr int kRows = 4;
+// A block takes 2048 neighbouring columns, eight per thread, and one strip of rows
+// (all of one gate vector), kRows rows' loads in flight at a time.  kVec: 16-byte
+// accesses (N, strides and addresses aligned); else single elements, a block's
+// width apart.
+//
+// Bound by HBM (dy and z in, dz out): 3456 x 12288 with GELU XX us of 39.5.  With
+// twelve instructions per value for the activation in scalar form it was bound by
+// issue (85 us), with two blocks per SM by the second wave (62 us).
+template <typename T, typename Z, bool kVec, int ACT>
+__global__ void __launch_bounds__(256, 3) dz_kernel(const DzParams p) {
+    constexpr int kRows = 2;
     pdl_launch_dependents();
     pdl_wait();
     const int64_t col_block = blockIdx.x % p.col_blocks, strip = blockIdx.x / p.col_blocks;
-    const int64_t c0 = (col_block * 256 + threadIdx.x) * V;
-    if (c0 >= p.N) return;
     const int64_t s = strip / p.strips_per_gate;
     const int64_t r_begin = s * p.rows_per_gate + strip % p.strips_per_gate * p.strip_rows;
-    const int64_t r_end = min(r_begin + p.strip_rows, (s + 1) * p.rows_per_gate);
-    struct alignas(sizeof(T) * V) Group {
-        T v[V];
-    };
-    struct alignas(V == 8 ? 16 : sizeof(Z)) GroupZ {
-        Z v[V];
-    };
-    const T* dyp = static_cast<const T*>(p.dy) + c0;
-    const Z* zp = static_cast<const Z*>(p.z) + c0;
-    Group gate{};
-    if (p.gate) gate = load_ro<Group>(static_cast<const T*>(p.gate) + s * p.ldg + c0);
-    float db[V], dg[V];
+    const int rows = static_cast<int>(min(p.strip_rows, (s + 1) * p.rows_per_gate - r_begin));
+    const int64_t c0 = col_block * 2048 + (kVec ? threadIdx.x * 8 : threadIdx.x);  // first column
+    if (c0 >= p.N) return;
+    const int left = static_cast<int>(min(p.N - c0, int64_t(2048)));  // strided: columns from c0 on in the block
+    auto load = [&](auto* row) {
+        using S = std::remove_cv_t<std::remove_pointer_t<decltype(row)>>;
+        Group<S, 8> g;
+        if constexpr (kVec) {
+            g = load_ro<Group<S, 8>>(row);
+        } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) db[i] = dg[i] = 0.0f;
-    for (int64_t r0 = r_begin; r0 < r_end; r0 += kRows) {
-        Group gy[kRows];
-        GroupZ gz[kRows];
+            for (int i = 0; i < 8; ++i) g.v[i] = 256 * i < left ? load_ro<S>(row + 256 * i) : from_f<S>(0.0f);
+        }
+        return g;
+    };
+    const T* dy = static_cast<const T*>(p.dy) + r_begin * p.ldy + c0;
+    const Z* z = p.z ? static_cast<const Z*>(p.z) + r_begin * p.N + c0 : nullptr;
+    T* dz = p.dz ? static_cast<T*>(p.dz) + r_begin * p.ldz + c0 : nullptr;
+    float2 gate[4], db[4], dg[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        gate[i] = both(1.0f);
+        db[i] = dg[i] = both(0.0f);
+    }
+    if (p.gate) unpack(load(static_cast<const T*>(p.gate) + s * p.ldg + c0), gate);
+    for (int r0 = 0; r0 < rows; r0 += kRows) {
+        Group<T, 8> gy[kRows];
+        Group<Z, 8> gz[kRows];
 #pragma unroll
         for (int k = 0; k < kRows; ++k) {
-            const int64_t r = min(r0 + k, r_end - 1);
-            gy[k] = load_ro<Group>(dyp + r * p.ldy);
-            if (p.z) gz[k] = load_ro<GroupZ>(zp + r * p.N);
+            const int64_t r = min(r0 + k, rows - 1);  // past the end: the last row again, not used
+            gy[k] = load(dy + r * p.ldy);
+            if (z) gz[k] = load(z + r * p.N);
         }
 #pragma unroll
         for (int k = 0; k < kRows; ++k) {
-            if (r0 + k < r_end) {
-                Group out;
+            if (r0 + k < rows) {
+                float2 fy[4], fz[4];
+                unpack(gy[k], fy);
+                if (z) unpack(gz[k], fz);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float dy = to_f(gy[k].v[i]);
-                    float a = 0.0f, slope = 1.0f;
-                    if (p.z) act_and_slope_f(to_f(gz[k].v[i]), ACT, a, slope);
-                    const float dz = (p.gate ? dy * to_f(gate.v[i]) : dy) * slope;
-                    db[i] += dz;
-                    dg[i] = fmaf(dy, a, dg[i]);
-                    out.v[i] = from_f<T>(dz);
+                for (int i = 0; i < 4; ++i) {
+                    float2 d = mul2(fy[i], gate[i]);
+                    if (z) {
+                        float2 a, slope;
+                        act_and_slope2<ACT>(fz[i], a, slope);
+                        dg[i] = fma2(fy[i], a, dg[i]);
+                        d = mul2(d, slope);
+                    }
+                    db[i] = add2(db[i], d);
+                    fy[i] = d;
                 }
-                if (p.dz) *reinterpret_cast<Group*>(static_cast<T*>(p.dz) + (r0 + k) * p.ldz + c0) = out;
+                if (dz) {
+                    const Group<T, 8> out = pack<T, 8>(fy);
+                    T* to = dz + int64_t(r0 + k) * p.ldz;
+                    if constexpr (kVec) {
+                        *reinterpret_cast<Group<T, 8>*>(to) = out;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (256 * i < left) to[256 * i] = out.v[i];
+                    }
+                }
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        if (p.db_part) p.db_part[strip * p.N + c0 + i] = db[i];
-        if (p.dg_part) p.dg_part[strip * p.N + c0 + i] = dg[i];
+    for (int which = 0; which < 2; ++which) {
+        float* part = which == 0 ? p.db_part : p.dg_part;
+        if (!part) continue;
+        part += strip * p.N + c0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 v = which == 0 ? db[i / 2] : dg[i / 2];
+            if (kVec || 256 * i < left) part[kVec ? i : 256 * i] = i & 1 ? v.y : v.x;
+        }
     }
 }
 
@@ -206,11 +241,10 @@ __global__ void __launch_bounds__(256) sum_strips_kernel(const float* db_part, c
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// Rows per strip: about four blocks per SM, strips of 4 rows at least.  One plan
-// for both access widths (the narrow one only has more column blocks).
+// Rows per strip: one wave of three blocks per SM, strips of 4 rows at least.
 void plan_strips(int64_t M, int64_t N, int64_t rows_per_gate, int64_t* strip_rows, int64_t* strips_per_gate) {
     const int64_t blocks = (N + 2047) / 2048 * (M / rows_per_gate);
-    const int64_t want = std::max<int64_t>(1, (int64_t(device_sm_count()) * 4 + blocks - 1) / blocks);
+    const int64_t want = std::max<int64_t>(1, int64_t(device_sm_count()) * 3 / blocks);
     *strip_rows = std::min(rows_per_gate, std::max<int64_t>(4, (rows_per_gate + want - 1) / want));
     *strips_per_gate = (rows_per_gate + *strip_rows - 1) / *strip_rows;
 }
@@ -220,13 +254,12 @@ int run_dz(DzParams p, int64_t M, void* dbias, void* dgate, cudaStream_t stream)
     const int64_t gates = M / p.rows_per_gate, strips = gates * p.strips_per_gate;
     const bool vec = p.N % 8 == 0 && p.ldy % 8 == 0 && (!p.gate || p.ldg % 8 == 0) && aligned16(p.dy) &&
                      aligned16(p.z) && aligned16(p.gate);
-    const int cols = vec ? 2048 : 256;
-    p.col_blocks = static_cast<unsigned>((p.N + cols - 1) / cols);
+    p.col_blocks = static_cast<unsigned>((p.N + 2047) / 2048);
     const int64_t db_blocks = dbias ? (p.N + 31) / 32 : 0, dg_blocks = dgate ? gates * ((p.N + 31) / 32) : 0;
     if (strips * p.col_blocks > kMaxGrid || db_blocks + dg_blocks > kMaxGrid) return Q6_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(strips * p.col_blocks));
-    const cudaError_t e = vec ? launch_pdl(dz_kernel<T, Z, 8, ACT>, grid, dim3(256), 0, stream, p)
-                              : launch_pdl(dz_kernel<T, Z, 1, ACT>, grid, dim3(256), 0, stream, p);
+    const cudaError_t e = vec ? launch_pdl(dz_kernel<T, Z, true, ACT>, grid, dim3(256), 0, stream, p)
+                              : launch_pdl(dz_kernel<T, Z, false, ACT>, grid, dim3(256), 0, stream, p);
     if (e != cudaSuccess) return Q6_ERR_CUDA;
     if (db_blocks + dg_blocks == 0) return Q6_OK;
     return launch_pdl(sum_strips_kernel<T>, dim3(static_cast<unsigned>(db_blocks + dg_blocks)), dim3(256), 0, stream,
@@ -265,7 +298,12 @@ struct Carver {
     }
 };
 
+// The few-row kernel reads its operands where they are; Q6_DENSE_PLAN (a plan of
+// the tensor-core path) turns it off.
+bool few_rows(int64_t M) { return M <= kDenseFewRows && !std::getenv("Q6_DENSE_PLAN"); }
+
 size_t forward_bytes(int64_t M, int64_t N, int64_t K, int pack) {
+    if (few_rows(M)) return 0;
     size_t b = round_up(dense_product_workspace_bytes(M, N, K, false, false));
     if (pack & Q6_PACK_X) b += round_up(size_t(M) * pad8(K) * 2);
     if (pack & Q6_PACK_W) b += round_up(size_t(N) * pad8(K) * 2);
@@ -346,29 +384,8 @@ int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     if (workspace && reinterpret_cast<uintptr_t>(workspace) % kAlign) return Q6_ERR_ALIGNMENT;
     const size_t need = forward_bytes(M, N, K, pack);
     if (need > (workspace ? workspace_bytes : 0)) return Q6_ERR_WORKSPACE;
-    Carver ws{static_cast<char*>(workspace)};
     DenseProduct a{};
-    a.workspace_bytes = dense_product_workspace_bytes(M, N, K, false, false);
-    a.workspace = ws.take(a.workspace_bytes);
-    Packer packer;
-    if (pack & Q6_PACK_X) {
-        void* c = ws.take(size_t(M) * pad8(K) * 2);
-        packer.add(x, ldx, c, M, K);
-        x = c;
-        ldx = pad8(K);
-    }
-    if (pack & Q6_PACK_W) {
-        void* c = ws.take(size_t(N) * pad8(K) * 2);
-        packer.add(w, ldw, c, N, K);
-        w = c;
-        ldw = pad8(K);
-    }
-    if (const int e = packer.launch(stream)) return e;
-    a.p = w;
-    a.ldp = ldw;
     a.p_t = false;
-    a.q = x;
-    a.ldq = ldx;
     a.q_t = false;
     a.d = y;
     a.R = M;
@@ -384,6 +401,31 @@ int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     a.epi.preact = preact;
     a.epi.preact_f32 = preact_dtype == Q6_DTYPE_F32;
     a.epi.activation = activation;
+    const bool rows = few_rows(M);
+    Carver ws{static_cast<char*>(workspace)};
+    if (!rows) {
+        a.workspace_bytes = dense_product_workspace_bytes(M, N, K, false, false);
+        a.workspace = ws.take(a.workspace_bytes);
+        Packer packer;
+        if (pack & Q6_PACK_X) {
+            void* c = ws.take(size_t(M) * pad8(K) * 2);
+            packer.add(x, ldx, c, M, K);
+            x = c;
+            ldx = pad8(K);
+        }
+        if (pack & Q6_PACK_W) {
+            void* c = ws.take(size_t(N) * pad8(K) * 2);
+            packer.add(w, ldw, c, N, K);
+            w = c;
+            ldw = pad8(K);
+        }
+        if (const int e = packer.launch(stream)) return e;
+    }
+    a.p = w;
+    a.ldp = ldw;
+    a.q = x;
+    a.ldq = ldx;
+    if (rows) return launch_dense_rows(a, stream);
     return launch_dense_product(a, stream);
 }
 

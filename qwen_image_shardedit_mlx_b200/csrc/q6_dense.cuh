@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "q6_b200.h"
 
 namespace q6 {
@@ -60,20 +62,6 @@ __device__ __forceinline__ float act_f(float z, int act) {
     return z * act_sigmoid(z, act, t);
 }
 
-// act(z) and act'(z) = s + z s (1 - s) du/dz, u the sigmoid's argument.
-__device__ __forceinline__ void act_and_slope_f(float z, int act, float& a, float& slope) {
-    if (act == Q6_ACT_NONE) {
-        a = z;
-        slope = 1.0f;
-        return;
-    }
-    float t;
-    const float s = act_sigmoid(z, act, t);
-    a = z * s;
-    const float q = a * (1.0f - s);
-    slope = act == Q6_ACT_GELU_TANH ? fmaf(q, fmaf(t, 3.0f * kGelu2K * kGeluC, kGelu2K), s) : q + s;
-}
-
 // 16-byte (or smaller) read-only loads: free to move across stores.
 template <typename S>
 __device__ __forceinline__ S load_ro(const void* p) {
@@ -91,6 +79,91 @@ __device__ __forceinline__ S load_ro(const void* p) {
         *reinterpret_cast<uint16_t*>(&out) = __ldg(static_cast<const uint16_t*>(p));
     }
     return out;
+}
+
+// Pairs of fp32 (packed arithmetic: half the instructions).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+template <typename T, int G>
+struct alignas(16) Group {
+    T v[G];
+};
+
+// A group's elements as pairs of fp32, and back.
+template <int G>
+__device__ __forceinline__ void unpack(const Group<__nv_bfloat16, G>& g, float2 (&f)[G / 2]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(g.v);
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+}
+template <int G>
+__device__ __forceinline__ void unpack(const Group<__half, G>& g, float2 (&f)[G / 2]) {
+    const __half2* w = reinterpret_cast<const __half2*>(g.v);
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) f[i] = __half22float2(w[i]);
+}
+template <int G>
+__device__ __forceinline__ void unpack(const Group<float, G>& g, float2 (&f)[G / 2]) {
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) f[i] = make_float2(g.v[2 * i], g.v[2 * i + 1]);
+}
+
+// A group from shared memory in one 16-byte load (read through a reference it
+// would be four 4-byte loads with four-way bank conflicts).
+template <typename T, int G>
+__device__ __forceinline__ Group<T, G> load_shared(const T* p) {
+    Group<T, G> g;
+    *reinterpret_cast<uint4*>(&g) = *reinterpret_cast<const uint4*>(p);
+    return g;
+}
+
+template <typename T, int G>
+__device__ __forceinline__ Group<T, G> pack(const float2 (&f)[G / 2]) {
+    Group<T, G> g;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) {
+            g.v[2 * i] = f[i].x;
+            g.v[2 * i + 1] = f[i].y;
+        }
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) reinterpret_cast<__half2*>(g.v)[i] = __floats2half2_rn(f[i].x, f[i].y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) reinterpret_cast<__nv_bfloat162*>(g.v)[i] = __floats2bfloat162_rn(f[i].x, f[i].y);
+    }
+    return g;
+}
+
+// act(z) = z s and act'(z) = s + z s (1 - s) du/dz, u the sigmoid's argument, on a
+// pair.
+template <int ACT>
+__device__ __forceinline__ void act_and_slope2(float2 z, float2& a, float2& slope) {
+    if constexpr (ACT == Q6_ACT_NONE) {
+        a = z;
+        slope = both(1.0f);
+    } else {
+        float2 t, arg;
+        if constexpr (ACT == Q6_ACT_GELU_TANH) {
+            t = mul2(z, z);
+            t = make_float2(fminf(t.x, 400.0f), fminf(t.y, 400.0f));
+            arg = mul2(z, fma2(t, both(-kLog2e * kGelu2K * kGeluC), both(-kLog2e * kGelu2K)));
+        } else {
+            arg = mul2(z, both(-kLog2e));
+        }
+        const float2 d = add2(make_float2(ex2_f(arg.x), ex2_f(arg.y)), both(1.0f));
+        const float2 s = make_float2(rcp_f(d.x), rcp_f(d.y));
+        a = mul2(z, s);
+        const float2 q = mul2(a, fma2(s, both(-1.0f), both(1.0f)));
+        if constexpr (ACT == Q6_ACT_GELU_TANH)
+            slope = fma2(q, fma2(t, both(3.0f * kGelu2K * kGeluC), both(kGelu2K)), s);
+        else
+            slope = add2(q, s);
+    }
 }
 
 }  // namespace q6

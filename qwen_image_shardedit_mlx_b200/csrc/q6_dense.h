@@ -40,6 +40,11 @@ struct DenseProduct {
     size_t workspace_bytes = 0;
 };
 
+// Up to kDenseFewRows rows of Q, both operands with the sum contiguous, any
+// alignment, no workspace (q6_dense_rows.cu).
+constexpr int64_t kDenseFewRows = 8;
+int launch_dense_rows(const DenseProduct& a, cudaStream_t stream);
+
 int launch_dense_product(const DenseProduct& a, cudaStream_t stream);
 size_t dense_product_workspace_bytes(int64_t R, int64_t C, int64_t L, bool p_t, bool q_t);
 

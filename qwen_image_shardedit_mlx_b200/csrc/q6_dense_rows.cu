@@ -1,0 +1,181 @@
+// Dense linear for a few rows (1 to 8): bound by reading the weight once.
+//
+//   y[m, n] = epilogue(sum_k x[m, k] W[n, k])
+//
+// A CTA takes 16 rows of W; its warps share the sum, 128 of k at a time.  The
+// products run on warp-level MMAs (m16n8k16) with the weight rows as the A operand
+// and the rows of x as B, straight from global memory: within a block of 32 of k
+// lane t of a row holds eight neighbouring values (one 16-byte load), and since
+// both operands number the sum's terms the same way, the MMA's own order of them
+// does not matter.  So the weight passes through no shared memory and no
+// shuffles; eight 16-byte loads of it per lane are in flight per turn.  The warps'
+// partial sums meet in shared memory and are added in order.
+//
+// bf16, one row: 3072 -> 18432 20.0 us (5.7 TB/s), 3072 -> 3072 6.2 us, 12288 -> 3072
+// 16.6 us; the tcgen05 path, which needs a second kernel for its split sums, takes
+// 20.9, 9.2 and 17.8.  At sixteen rows x is read as often as the weight and the
+// tcgen05 path wins (3072 -> 3072 9.4 against 11.4 us), so this one ends at eight.
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "q6_dense.cuh"
+#include "q6_dense.h"
+#include "q6_internal.h"
+#include "q6_ptx.cuh"
+
+namespace q6 {
+namespace {
+
+constexpr int kTileN = 16;     // weight rows per CTA
+constexpr int kBlocks = 4;     // blocks of 32 of k per turn
+constexpr int kTurn = 32 * kBlocks;
+constexpr int kMaxWarps = 16;
+constexpr int kMost = static_cast<int>(kDenseFewRows);
+
+struct RowsParams {
+    const void* x;
+    const void* w;
+    void* y;
+    int64_t ldx, ldw;
+    int M, N, K;
+    int gate_rows;
+    DenseEpilogue epi;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight values of a row from k on, zero past K; kBytes: what the row's alignment
+// allows per load (16, 4 or 2).
+template <int kBytes>
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (kBytes == 16) {
+        if (k < K) v = __ldg(reinterpret_cast<const uint4*>(row + k));
+    } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kBytes == 4) {
+                if (k + 2 * i < K) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row + k + 2 * i));
+            } else {
+                const uint32_t lo = k + 2 * i < K ? __ldg(row + k + 2 * i) : 0u;
+                const uint32_t hi = k + 2 * i + 1 < K ? __ldg(row + k + 2 * i + 1) : 0u;
+                w[i] = lo | hi << 16;
+            }
+        }
+    }
+    return v;
+}
+
+template <typename T, int kBytes>
+__global__ void __launch_bounds__(kMaxWarps * 32) dense_rows_kernel(const RowsParams p) {
+    static_assert(kMost == 8, "one MMA tile of rows of x");
+    __shared__ float sums[kMaxWarps][kMost][kTileN + 1];
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * kTileN;
+    // rows beyond the weight read its last one and are not stored; rows beyond x are zeros
+    const uint16_t* w0 = static_cast<const uint16_t*>(p.w) + int64_t(min(n0 + g, p.N - 1)) * p.ldw;
+    const uint16_t* w1 = static_cast<const uint16_t*>(p.w) + int64_t(min(n0 + g + 8, p.N - 1)) * p.ldw;
+    const uint16_t* x = static_cast<const uint16_t*>(p.x) + g * p.ldx;
+    pdl_wait();
+    float c[4] = {};
+    for (int k0 = warp * kTurn; k0 < p.K; k0 += warps * kTurn) {
+        uint4 a0[kBlocks], a1[kBlocks], b[kBlocks];
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int k = k0 + 32 * i + 8 * t;
+            a0[i] = load8<kBytes>(w0, k, p.K);
+            a1[i] = load8<kBytes>(w1, k, p.K);
+        }
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            b[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (g < p.M) b[i] = load8<kBytes>(x, k0 + 32 * i + 8 * t, p.K);
+        }
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            mma16816<T>(c, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
+            mma16816<T>(c, a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
+        }
+    }
+    // c: weight rows g and g + 8, rows 2 t and 2 t + 1 of x
+    sums[warp][2 * t][g] = c[0];
+    sums[warp][2 * t + 1][g] = c[1];
+    sums[warp][2 * t][g + 8] = c[2];
+    sums[warp][2 * t + 1][g + 8] = c[3];
+    __syncthreads();
+    const DenseEpilogue& e = p.epi;
+    for (int i = threadIdx.x; i < p.M * kTileN; i += blockDim.x) {
+        const int m = i / kTileN, n = n0 + i % kTileN;
+        if (n >= p.N) continue;
+        float v = 0.0f;
+        for (int k = 0; k < warps; ++k) v += sums[k][m][i % kTileN];
+        if (e.bias) v += to_f(static_cast<const T*>(e.bias)[n]);
+        const int64_t at = int64_t(m) * p.N + n;
+        if (e.preact) {
+            if (e.preact_f32)
+                static_cast<float*>(e.preact)[at] = v;
+            else
+                static_cast<T*>(e.preact)[at] = from_f<T>(v);
+        }
+        v = act_f(v, e.activation);
+        if (e.gate) v *= to_f(static_cast<const T*>(e.gate)[m / p.gate_rows * e.ldg + n]);
+        if (e.residual) v += to_f(static_cast<const T*>(e.residual)[m * e.ldr + n]);
+        static_cast<T*>(p.y)[at] = from_f<T>(v);
+    }
+}
+
+template <typename T>
+cudaError_t launch_typed(const RowsParams& p, int bytes, cudaStream_t stream) {
+    // about 16 warps per SM in all, no more than the turns of one sum
+    const int64_t tiles = (p.N + kTileN - 1) / kTileN, turns = (p.K + kTurn - 1) / kTurn;
+    const int64_t want = (int64_t(device_sm_count()) * 16 + tiles - 1) / tiles;
+    const int64_t warps = std::max<int64_t>(1, std::min<int64_t>({want, turns, int64_t(kMaxWarps)}));
+    const dim3 grid(static_cast<unsigned>(tiles)), block(static_cast<unsigned>(32 * warps));
+    if (bytes == 16) return launch_pdl(dense_rows_kernel<T, 16>, grid, block, 0, stream, p);
+    if (bytes == 4) return launch_pdl(dense_rows_kernel<T, 4>, grid, block, 0, stream, p);
+    return launch_pdl(dense_rows_kernel<T, 2>, grid, block, 0, stream, p);
+}
+
+}  // namespace
+
+int launch_dense_rows(const DenseProduct& a, cudaStream_t stream) {
+    RowsParams p{};
+    p.x = a.q;
+    p.w = a.p;
+    p.y = a.d;
+    p.ldx = a.ldq;
+    p.ldw = a.ldp;
+    p.M = static_cast<int>(a.R);
+    p.N = static_cast<int>(a.C);
+    p.K = static_cast<int>(a.L);
+    p.gate_rows = a.epi.gate ? static_cast<int>(a.epi.rows_per_gate) : p.M;
+    p.epi = a.epi;
+    const auto fits = [&](int64_t bytes) {
+        const int64_t e = bytes / 2;
+        return p.K % e == 0 && p.ldw % e == 0 && p.ldx % e == 0 && reinterpret_cast<uintptr_t>(p.w) % bytes == 0 &&
+               reinterpret_cast<uintptr_t>(p.x) % bytes == 0;
+    };
+    const int bytes = fits(16) ? 16 : fits(4) ? 4 : 2;
+    const cudaError_t e = a.dtype == Q6_DTYPE_F16 ? launch_typed<__half>(p, bytes, stream)
+                                                  : launch_typed<__nv_bfloat16>(p, bytes, stream);
+    return e == cudaSuccess ? Q6_OK : Q6_ERR_CUDA;
+}
+
+}  // namespace q6

@@ -62,63 +62,6 @@ struct NormParams {
 
 namespace norm_detail {
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
-template <typename T, int G>
-struct alignas(16) Group {
-    T v[G];
-};
-
-// A group's elements as pairs of fp32, and back.
-template <int G>
-__device__ __forceinline__ void unpack(const Group<__nv_bfloat16, G>& g, float2 (&f)[G / 2]) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(g.v);
-#pragma unroll
-    for (int i = 0; i < G / 2; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
-}
-template <int G>
-__device__ __forceinline__ void unpack(const Group<__half, G>& g, float2 (&f)[G / 2]) {
-    const __half2* w = reinterpret_cast<const __half2*>(g.v);
-#pragma unroll
-    for (int i = 0; i < G / 2; ++i) f[i] = __half22float2(w[i]);
-}
-template <int G>
-__device__ __forceinline__ void unpack(const Group<float, G>& g, float2 (&f)[G / 2]) {
-#pragma unroll
-    for (int i = 0; i < G / 2; ++i) f[i] = make_float2(g.v[2 * i], g.v[2 * i + 1]);
-}
-
-// A group from shared memory in one 16-byte load (read through a reference it
-// would be four 4-byte loads with four-way bank conflicts).
-template <typename T, int G>
-__device__ __forceinline__ Group<T, G> load_shared(const T* p) {
-    Group<T, G> g;
-    *reinterpret_cast<uint4*>(&g) = *reinterpret_cast<const uint4*>(p);
-    return g;
-}
-
-template <typename T, int G>
-__device__ __forceinline__ Group<T, G> pack(const float2 (&f)[G / 2]) {
-    Group<T, G> g;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < G / 2; ++i) {
-            g.v[2 * i] = f[i].x;
-            g.v[2 * i + 1] = f[i].y;
-        }
-    } else if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-        for (int i = 0; i < G / 2; ++i) reinterpret_cast<__half2*>(g.v)[i] = __floats2half2_rn(f[i].x, f[i].y);
-    } else {
-#pragma unroll
-        for (int i = 0; i < G / 2; ++i) reinterpret_cast<__nv_bfloat162*>(g.v)[i] = __floats2bfloat162_rn(f[i].x, f[i].y);
-    }
-    return g;
-}
-
 // Sum over the 32 lanes of each of v's two values, in every lane: the first
 // exchange leaves one value per lane, so two sums cost six shuffles.
 __device__ __forceinline__ float2 warp_sum2(float2 v) {

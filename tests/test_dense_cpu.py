@@ -106,8 +106,8 @@ def test_c_entries_refuse_before_the_device():
     assert linear(act=3) == inv and linear(act=-1) == inv
     assert linear(dtype=2) == uns and linear(pre=256, pdt=1) == uns and linear(pre=258, pdt=2) == al
     assert linear(x=257) == al and linear(y=255) == al and linear(ws=128, wsb=1 << 30) == al
-    assert linear(x=258) == wsp  # an operand off its 16 bytes is copied: the workspace must hold it
-    assert lib.q6_dense_linear_workspace_bytes(4, 32, 64, _lib.Q6_PACK_X) >= 4 * 64 * 2
+    assert linear(M=40, rpg=40, x=258) == wsp  # an operand off its 16 bytes is copied: the workspace must hold it
+    assert lib.q6_dense_linear_workspace_bytes(40, 32, 64, _lib.Q6_PACK_X) >= 40 * 64 * 2
     assert lib.q6_dense_linear_workspace_bytes(0, 32, 64, 0) == 0
 
     def grad(**kw):
