@@ -65,7 +65,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Tile shape and split of one product: the least estimated time over the tile
 // shapes.  In cycles: a stage costs the longer of its MMAs (2 CT per 64 of
 // depth) and its operand bytes at 44 a cycle; a work item 700 more (ring fill,
-// epilogue hand-over), a split the second kernel and its partials' traffic.
+// epilogue hand-over), a split the second kernel and its partials' traffic.  (A
+// split joined within a cluster, each CTA's tile left in its shared memory, took
+// as long: 9.5 us at 16 x 3072 -> 3072, 28 us at 256 x 12288 -> 3072.)
 DensePlan plan_dense(int64_t R, int64_t C, int64_t L, bool q_t) {
     const int64_t sms = device_sm_count();
     struct Shape {
@@ -98,7 +100,7 @@ DensePlan plan_dense(int64_t R, int64_t C, int64_t L, bool q_t) {
             if (ceil_div(stages, per) != s) continue;
             const int64_t waves = ceil_div(tiles * s, units);
             double cost = waves * (per * stage + 700.0) + 2.0 * sh.ct;
-            if (s > 1) cost += 4000.0 + static_cast<double>(s) * R * C * 4 / 2500.0;
+            if (s > 1) cost += 5000.0 + s * (700.0 + R * C * 4 / 1500.0);
             if (best.ct == 0 || cost < best_cost) {
                 best_cost = cost;
                 best = DensePlan{sh.ct, sh.pair, static_cast<int>(s), static_cast<int>(per)};

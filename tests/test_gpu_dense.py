@@ -118,6 +118,26 @@ def test_linear_every_contraction_length(k):
     check_linear(*make_linear(1, 3, k, 80, torch.bfloat16, seed=k), None)
 
 
+PLANS = [f"{ct},{pair},{split}" for ct, pair in ((256, 1), (192, 1), (128, 1), (128, 0), (64, 0), (32, 0), (16, 0))
+         for split in (1, 2, 3, 4, 8, 11)]
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_linear_every_tile_shape_and_split(plan, monkeypatch):
+    # every tile shape, alone and with the sum split, at sizes that
+    # leave ragged tiles on every side, in every operand order (forward, dx, dw)
+    monkeypatch.setenv("Q6_DENSE_PLAN", plan)
+    check_linear(*make_linear(2, 150, 808, 696, torch.bfloat16), "gelu_tanh")
+    check_linear(*make_linear(1, 515, 707, 773, torch.float16, gate=False), "silu")
+    check_linear(*make_linear(1, 5, 1544, 264, torch.bfloat16), None)
+
+
+@pytest.mark.parametrize("shape", [(1, 3456, 768, 3072), (2, 1728, 3072, 776), (1, 4099, 1031, 515), (3, 700, 520, 2056)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_linear_large(shape):
+    check_linear(*make_linear(*shape, torch.bfloat16), "gelu_tanh")
+
+
 def test_linear_strided_views_and_odd_addresses():
     dtype = torch.bfloat16
     base = rand((2, 70, 400), dtype, 1)
