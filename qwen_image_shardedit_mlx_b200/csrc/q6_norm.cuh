@@ -164,21 +164,19 @@ struct Columns {
 // Forward: W warps per row (one row per CTA; four with W = 1), N groups per
 // thread.  N is at most four: a row's code runs once per row, and with twelve
 // groups per lane (a warp per row of 3072) its unrolled length ran out of the
-// instruction cache: 31 us for 6912 rows of bf16 against 21 us with four.
+// instruction cache: 31 us for 6912 rows of bf16 against 21 us with four.  The
+// grid is one wave of CTAs that walk the rows, the next row's loads in flight
+// while a row is summed: 15.7 us (5.4 TB/s).
 template <typename T, typename V, Layout kLay, int W, int N>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormParams p) {
     constexpr int G = 16 / sizeof(T), kRows = W == 1 ? 4 : 1;
     __shared__ float parts[2][W];
     pdl_launch_dependents();
-    const int64_t local = W == 1 ? blockIdx.x * int64_t(kRows) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
-    if (local >= (p.vecs ? p.rows_per_vec : p.M)) return;  // a whole warp of a CTA of single-warp rows
-    int64_t row = local, v0 = 0;
-    if (p.vecs) {
-        row += blockIdx.y * p.rows_per_vec;
-        v0 = blockIdx.y * p.ldv;
-    } else if (p.rows_per_vec < p.M) {
-        v0 = row / p.rows_per_vec * p.ldv;
-    }
+    // rows first, first + step, ... of a vector's rows, or of all where the vectors are not the grid's second axis
+    const int64_t limit = p.vecs ? p.rows_per_vec : p.M, step = gridDim.x * int64_t(kRows);
+    int64_t local = W == 1 ? blockIdx.x * int64_t(kRows) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
+    if (local >= limit) return;  // a whole warp of a CTA of single-warp rows
+    const int64_t row0 = p.vecs ? blockIdx.y * p.rows_per_vec : 0;
     pdl_wait();
     const Columns<T, kLay, 32 * W> at{W == 1 ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
                                       static_cast<int>(p.D)};
@@ -193,57 +191,75 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormP
         }
         return v;
     };
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* x = static_cast<const T*>(p.x) + (row0 + local) * p.ldx;
     Group<T, G> in[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) in[j] = at.load(x, j);
-    const V* w = p.weight ? static_cast<const V*>(p.weight) + v0 : nullptr;
-    const V* b = p.bias ? static_cast<const V*>(p.bias) + v0 : nullptr;
-    float2 c[N][G / 2];
-    float2 s = both(0.0f);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (at.some(j)) {
-            unpack(in[j], c[j]);
-#pragma unroll
-            for (int i = 0; i < G / 2; ++i) s = add2(s, c[j][i]);
-        }
-    }
     const float inv = 1.0f / static_cast<float>(at.D);
-    const float mean = row_sum(s.x + s.y, 0) * inv;
-    float2 q = both(0.0f);
+    for (;; local += step) {
+        const int64_t row = row0 + local;
+        const bool more = local + step < limit;
+        Group<T, G> next[N];
+        if (more) {
+            x += step * p.ldx;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (at.some(j)) {
+            for (int j = 0; j < N; ++j) next[j] = at.load(x, j);
+        }
+        int64_t v0 = 0;
+        if (p.vecs)
+            v0 = blockIdx.y * p.ldv;
+        else if (p.rows_per_vec < p.M)
+            v0 = row / p.rows_per_vec * p.ldv;
+        const V* w = p.weight ? static_cast<const V*>(p.weight) + v0 : nullptr;
+        const V* b = p.bias ? static_cast<const V*>(p.bias) + v0 : nullptr;
+        float2 c[N][G / 2];
+        float2 s = both(0.0f);
 #pragma unroll
-            for (int i = 0; i < G / 2; ++i) {
-                c[j][i] = add2(c[j][i], both(-mean));
-                if constexpr (kLay == kStrided) {
-                    if (!at.inside(j, 2 * i)) c[j][i].x = 0.0f;
-                    if (!at.inside(j, 2 * i + 1)) c[j][i].y = 0.0f;
-                }
-                q = fma2(c[j][i], c[j][i], q);
+        for (int j = 0; j < N; ++j) {
+            if (at.some(j)) {
+                unpack(in[j], c[j]);
+#pragma unroll
+                for (int i = 0; i < G / 2; ++i) s = add2(s, c[j][i]);
             }
         }
-    }
-    const float rstd = rsqrtf(row_sum(q.x + q.y, 1) * inv + p.eps);
-    if (p.mean && at.t == 0) {
-        p.mean[row] = mean;
-        p.rstd[row] = rstd;
-    }
-    T* y = static_cast<T*>(p.y) + row * p.D;
+        const float mean = row_sum(s.x + s.y, 0) * inv;
+        float2 q = both(0.0f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (at.some(j)) {
-            float2 fw[G / 2], fb[G / 2];
-            at.factor(w, j, p.one, fw);
+        for (int j = 0; j < N; ++j) {
+            if (at.some(j)) {
 #pragma unroll
-            for (int i = 0; i < G / 2; ++i) fb[i] = both(0.0f);
-            if (b) unpack(at.load(b, j), fb);
-#pragma unroll
-            for (int i = 0; i < G / 2; ++i) fb[i] = fma2(mul2(c[j][i], both(rstd)), fw[i], fb[i]);
-            at.store(y, j, pack<T, G>(fb));
+                for (int i = 0; i < G / 2; ++i) {
+                    c[j][i] = add2(c[j][i], both(-mean));
+                    if constexpr (kLay == kStrided) {
+                        if (!at.inside(j, 2 * i)) c[j][i].x = 0.0f;
+                        if (!at.inside(j, 2 * i + 1)) c[j][i].y = 0.0f;
+                    }
+                    q = fma2(c[j][i], c[j][i], q);
+                }
+            }
         }
+        const float rstd = rsqrtf(row_sum(q.x + q.y, 1) * inv + p.eps);
+        if (p.mean && at.t == 0) {
+            p.mean[row] = mean;
+            p.rstd[row] = rstd;
+        }
+        T* y = static_cast<T*>(p.y) + row * p.D;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (at.some(j)) {
+                float2 fw[G / 2], fb[G / 2];
+                at.factor(w, j, p.one, fw);
+#pragma unroll
+                for (int i = 0; i < G / 2; ++i) fb[i] = both(0.0f);
+                if (b) unpack(at.load(b, j), fb);
+#pragma unroll
+                for (int i = 0; i < G / 2; ++i) fb[i] = fma2(mul2(c[j][i], both(rstd)), fw[i], fb[i]);
+                at.store(y, j, pack<T, G>(fb));
+            }
+        }
+        if (!more) return;
+#pragma unroll
+        for (int j = 0; j < N; ++j) in[j] = next[j];
     }
 }
 
@@ -636,10 +652,23 @@ int norm_grad_typed(const NormParams& p, bool vec, int shape, V* dweight, V* dbi
 
 template <typename T, typename V, norm_detail::Layout kLay, int W, int N>
 int launch_norm_forward(const NormParams& p, cudaStream_t stream) {
-    const int64_t rows = p.vecs ? p.rows_per_vec : p.M, per = W == 1 ? 4 : 1;
-    return launch_pdl(norm_detail::norm_kernel<T, V, kLay, W, N>,
-                      dim3(static_cast<unsigned>((rows + per - 1) / per), p.vecs ? p.vecs : 1u),
-                      dim3(W == 1 ? 128 : 32 * W), 0, stream, p) == cudaSuccess
+    auto* kernel = norm_detail::norm_kernel<T, V, kLay, W, N>;
+    constexpr int threads = W == 1 ? 128 : 32 * W;
+    // CTAs per SM, looked up once per device
+    static std::atomic<int> resident[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return Q6_ERR_CUDA;
+    if (dev < 0 || dev >= kMaxDevices) return Q6_ERR_UNSUPPORTED;
+    int per_sm = resident[dev].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1)
+            return Q6_ERR_CUDA;
+        resident[dev].store(per_sm, std::memory_order_relaxed);
+    }
+    const int64_t rows = p.vecs ? p.rows_per_vec : p.M, vecs = p.vecs ? p.vecs : 1, per = W == 1 ? 4 : 1;
+    const int64_t wave = std::max<int64_t>(1, int64_t(device_sm_count()) * per_sm / vecs);
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(std::min((rows + per - 1) / per, wave)), p.vecs ? p.vecs : 1u),
+                      dim3(threads), 0, stream, p) == cudaSuccess
                ? Q6_OK
                : Q6_ERR_CUDA;
 }

@@ -498,3 +498,173 @@ def test_feed_forward_half_forward_and_backward(dtype):
                             (ggate, dgate, "dgate"), (gw1, dw1, "dw1"), (gb1, db1, "db1"), (gw2, dw2, "dw2"),
                             (gb2, db2, "db2")):
         want.check(got.reshape(want.v.shape), name)
+
+
+def make_ff(d=128, h=256, seed=0):
+    from qwen_image_shardedit_mlx_b200 import QwenFeedForward
+
+    return QwenFeedForward.random(d, h, generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def test_materialised_feed_forward_half_trains():
+    from qwen_image_shardedit_mlx_b200.dense_img_ff_window import materialize_dense_img_ff
+
+    s, t, d = 2, 40, 128
+    ff, _ = materialize_dense_img_ff(make_ff())
+    x, dy = rand((s, t, d), torch.bfloat16, 1), rand((s, t, d), torch.bfloat16, 2)
+    shift, scale, gate = (rand((s, d), torch.bfloat16, 3 + i, 0.3) for i in range(3))
+    weights = [ff.mlp_in.weight, ff.mlp_in.bias, ff.mlp_out.weight, ff.mlp_out.bias]
+    leaves = [x, shift, scale, gate, *weights]
+    for leaf in leaves:
+        leaf.requires_grad_(True)
+    y = ff.half(x, shift, scale, gate)
+    grads = torch.autograd.grad(y, leaves, dy)
+    # the same calls one by one, without autograd: the same bits
+    with torch.no_grad():
+        h, mean, rstd = dense.layer_norm_modulate_forward(x, shift, scale)
+        a, z1 = dense.dense_linear_forward(h, weights[0], weights[1], activation="gelu_tanh", save_preact=True)
+        out, z2 = dense.dense_linear_forward(a, weights[2], weights[3], residual=x, gate=gate, save_preact=True)
+        g2 = dense.dense_linear_backward(dy, a, weights[2], preact=z2, gate=gate,
+                                         outputs=("x", "weight", "bias", "gate"))
+        g1 = dense.dense_linear_backward(g2.x, h, weights[0], preact=z1, activation="gelu_tanh")
+        gn = dense.layer_norm_modulate_backward(g1.x, x, scale, mean, rstd)
+    assert torch.equal(y, out)
+    for got, want in zip(grads, (gn.x + dy, gn.bias, gn.weight, g2.gate, g1.weight, g1.bias, g2.weight, g2.bias)):
+        assert torch.equal(got, want)
+    # the unfused module rounds where the fused one does not: its own roundings (the
+    # products' outputs, the bias sums, GELU) bound the distance
+    with torch.no_grad():
+        fused, plain = ff.fused(x).double(), ff(x).double()
+    assert (fused - plain).norm() <= 4 * 2.0 ** -8 * plain.norm()
+
+
+def test_materialised_feed_forward_with_an_adapter():
+    from qwen_image_shardedit_mlx_b200.dense_img_ff_window import materialize_dense_img_ff
+    from qwen_image_shardedit_mlx_b200.lora import iter_adapters, lora_delta_weight
+
+    q6 = make_ff()
+    a, b = rand((128, 32), torch.bfloat16, 5, 0.1), rand((32, 256), torch.bfloat16, 6, 0.1)
+    q6.mlp_in.set_lora(a, b, 0.5)
+    additive, _ = materialize_dense_img_ff(q6)
+    x = rand((3, 128), torch.bfloat16, 7)
+    with pytest.raises(ValueError, match="fold_single"):
+        additive.fused(x)
+    folded, _ = materialize_dense_img_ff(q6, fold_single=True)
+    assert folded.mlp_in_lora is None
+    q6.mlp_in.set_lora(None)
+    base, _ = materialize_dense_img_ff(q6)
+    q6.mlp_in.set_lora(a, b, 0.5)
+    want = (base.mlp_in.weight.float() + lora_delta_weight(list(iter_adapters(q6.mlp_in)), dtype=torch.float32)
+            ).to(torch.bfloat16)
+    assert torch.equal(folded.mlp_in.weight, want)
+    assert folded.fused(x).shape == (3, 128)
+
+
+def test_second_derivatives_are_refused():
+    x = rand((4, 16), torch.bfloat16, 1).requires_grad_(True)
+    w = rand((8, 16), torch.bfloat16, 2).requires_grad_(True)
+    for y in (dense.dense_linear(x, w, activation="silu"), dense.layer_norm(x)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_saved_tensors_changed_in_place_are_noticed():
+    x = rand((4, 16), torch.bfloat16, 1)
+    w = rand((8, 16), torch.bfloat16, 2).requires_grad_(True)
+    y = dense.dense_linear(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_gradients_add_up_over_calls_that_share_leaves():
+    x = rand((2, 24, 32), torch.bfloat16, 1)
+    w = rand((32, 32), torch.bfloat16, 2, 0.2).requires_grad_(True)
+    v = rand((32,), torch.float32, 3).requires_grad_(True)
+    one, = torch.autograd.grad(dense.dense_linear(x, w).float().sum(), w)
+    (dense.dense_linear(x, w).float().sum() + dense.dense_linear(x, w).float().sum()).backward()
+    assert torch.equal(w.grad, one + one)
+    h = dense.layer_norm(dense.dense_linear(dense.layer_norm(x, v), w), v)  # the same vector in two norms
+    h.float().sum().backward()
+    assert v.grad.shape == (32,) and v.grad.isfinite().all()
+
+
+def test_operators_on_a_side_stream_with_tensors_of_another():
+    x, w, b, g, r, dy = make_linear(2, 70, 136, 264, torch.bfloat16)
+    ready = torch.cuda.Event()
+    ready.record()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_event(ready)
+        w.requires_grad_(True)
+        y = dense.dense_linear(x, w, b, activation="silu", residual=r, gate=g)
+        n = dense.layer_norm(y, None, None)
+        grad, = torch.autograd.grad(n, w, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    y2 = dense.dense_linear(x, w, b, activation="silu", residual=r, gate=g)
+    grad2, = torch.autograd.grad(dense.layer_norm(y2), w, dy)
+    assert torch.equal(y, y2) and torch.equal(grad, grad2)
+
+
+def test_rows_far_into_a_tensor_of_more_than_2_31_elements():
+    # a view whose rows start past 2^31 elements: offsets are 64-bit
+    d, rows = 1 << 20, 2100
+    big = torch.zeros((rows, d), dtype=torch.bfloat16, device="cuda")
+    x = big[rows - 3:, 5:5 + 264]
+    x.copy_(rand((3, 264), torch.bfloat16, 1))
+    near = x.contiguous()
+    w = rand((72, 264), torch.bfloat16, 2, 0.1)
+    assert torch.equal(dense.dense_linear(x, w), dense.dense_linear(near, w))
+    assert torch.equal(dense.layer_norm(x), dense.layer_norm(near))
+    wide = big[::700, :264]  # rows 7.3e8 elements apart
+    wide.copy_(rand(wide.shape, torch.bfloat16, 3))
+    pad = wide.contiguous()
+    assert torch.equal(dense.layer_norm(wide), dense.layer_norm(pad))
+    tall = torch.cat([wide.contiguous()] * 4)
+    many = big[::175, 8:272]
+    many.copy_(tall[:many.shape[0]] if many.shape[0] <= tall.shape[0] else many)
+    assert torch.equal(dense.dense_linear(many, w), dense.dense_linear(many.contiguous(), w))
+
+
+def test_outputs_of_more_than_2_31_elements():
+    m, k, n = 131080, 8, 16400  # 2.15e9 outputs
+    x, w = rand((m, k), torch.bfloat16, 1), rand((n, k), torch.bfloat16, 2)
+    y = dense.dense_linear(x, w)
+    for rows in (slice(0, 5), slice(m // 2, m // 2 + 5), slice(m - 5, m)):
+        assert torch.equal(y[rows], dense.dense_linear(x[rows].contiguous(), w))
+    del y
+    d = 1 << 15
+    x = torch.zeros((65600, d), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = rand((3, d), torch.bfloat16, 3)
+    y = dense.layer_norm(x)
+    assert torch.equal(y[-3:], dense.layer_norm(x[-3:].contiguous()))
+
+
+def test_padded_batch_leaves_the_padding_alone():
+    # rows behind the last one of a buffer stay as they were
+    x, w, b, _, _, _ = make_linear(1, 45, 72, 96, torch.bfloat16, gate=False)
+    y = dense.dense_linear(x[0, :37], w, b)
+    after = torch.full((16, 96), 3.0, dtype=torch.bfloat16, device="cuda")
+    assert y.shape == (37, 96) and torch.equal(after, torch.full_like(after, 3.0))
+    assert torch.equal(y, dense.dense_linear(x, w, b)[0, :37])
+
+
+@pytest.mark.parametrize("samples,rows", [(70000, 1), (300, 3), (64, 100)])
+def test_many_vectors(samples, rows):
+    x, w, b, dy = make_norm(samples, rows, 24, torch.bfloat16, torch.bfloat16, per_sample=True)
+    check_norm(x, w, b, dy, modulate=True)
+
+
+def test_many_gates():
+    check_linear(*make_linear(700, 3, 40, 56, torch.bfloat16), "silu")
+    check_linear(*make_linear(3000, 1, 8, 24, torch.float16), None)
+
+
+def test_status_errors_have_the_library_class():
+    from qwen_image_shardedit_mlx_b200._lib import Q6Error
+
+    x = torch.zeros((2, 8), dtype=torch.bfloat16, device="cuda")
+    huge = torch.zeros((1,), dtype=torch.bfloat16, device="cuda").expand((1 << 30) + 1, 1)[:, :1]
+    with pytest.raises(Q6Error):
+        dense.dense_linear_forward(huge, torch.zeros((1, 1), dtype=torch.bfloat16, device="cuda"))
+    assert dense.dense_linear(x, x).shape == (2, 2)
