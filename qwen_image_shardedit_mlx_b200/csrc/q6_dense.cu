@@ -114,7 +114,7 @@ struct DzParams {
 // accesses (N, strides and addresses aligned); else single elements, a block's
 // width apart.
 //
-// Bound by HBM (dy and z in, dz out): 3456 x 12288 with GELU XX us of 39.5.  With
+// Bound by HBM (dy and z in, dz out): 3456 x 12288 with GELU 46 us of 39.5.  With
 // twelve instructions per value for the activation in scalar form it was bound by
 // issue (85 us), with two blocks per SM by the second wave (62 us).
 template <typename T, typename Z, bool kVec, int ACT>

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) dense_reduce_kernel(const DenseParams p) 
             float v[1] = {0.0f};
             for (int s = 0; s < p.splits; ++s) v[0] += src[s * plane];
             const float bias = p.epi.bias ? to_f(static_cast<const T*>(p.epi.bias)[c]) : 0.0f;
-            finish_column<T, 1>(p.epi, p.d, r, 1, p.C, c, p.gate_rows, bias, v);
+            finish_column<T, 1, false>(p.epi, p.d, r, 1, p.C, c, p.gate_rows, bias, v);
         }
     }
 }

@@ -202,33 +202,40 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
 }
 
 // The same for kRows outputs of one column c (rows r .. r + n - 1 of them), any
-// layout; the rows' loads are issued together.
-template <typename T, int kRows>
+// layout; the rows' loads are issued together.  kPlain: a bias at most.
+template <typename T, int kRows, bool kPlain>
 __device__ __forceinline__ void finish_column(const DenseEpilogue& e, void* d, int r, int n, int64_t C, int c,
                                               int gate_rows, float bias, float (&v)[kRows]) {
-    T res[kRows], gate[kRows];
+    T* y = static_cast<T*>(d) + r * C + c;
+    if constexpr (kPlain) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        if (i < n) {
-            if (e.residual) res[i] = static_cast<const T*>(e.residual)[(r + i) * e.ldr + c];
-            if (e.gate) gate[i] = static_cast<const T*>(e.gate)[(r + i) / gate_rows * e.ldg + c];
-        }
-    }
-    int64_t at = r * C + c;
+        for (int i = 0; i < kRows; ++i, y += C)
+            if (i < n) *y = from_f<T>(v[i] + bias);
+    } else {
+        T res[kRows], gate[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i, at += C) {
-        if (i < n) {
-            float t = v[i] + bias;
-            if (e.preact) {
-                if (e.preact_f32)
-                    static_cast<float*>(e.preact)[at] = t;
-                else
-                    static_cast<T*>(e.preact)[at] = from_f<T>(t);
+        for (int i = 0; i < kRows; ++i) {
+            if (i < n) {
+                if (e.residual) res[i] = static_cast<const T*>(e.residual)[(r + i) * e.ldr + c];
+                if (e.gate) gate[i] = static_cast<const T*>(e.gate)[(r + i) / gate_rows * e.ldg + c];
             }
-            t = act_f(t, e.activation);
-            if (e.gate) t *= to_f(gate[i]);
-            if (e.residual) t += to_f(res[i]);
-            static_cast<T*>(d)[at] = from_f<T>(t);
+        }
+        int64_t at = r * C + c;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i, at += C, y += C) {
+            if (i < n) {
+                float t = v[i] + bias;
+                if (e.preact) {
+                    if (e.preact_f32)
+                        static_cast<float*>(e.preact)[at] = t;
+                    else
+                        static_cast<T*>(e.preact)[at] = from_f<T>(t);
+                }
+                t = act_f(t, e.activation);
+                if (e.gate) t *= to_f(gate[i]);
+                if (e.residual) t += to_f(res[i]);
+                *y = from_f<T>(t);
+            }
         }
     }
 }
@@ -284,12 +291,17 @@ __device__ __forceinline__ void dense_epilogue_block(const DenseParams& p, const
         const int c = c0 + lane;
         if (c < p.C) {
             const float b = e.bias ? to_f(static_cast<const T*>(e.bias)[c]) : 0.0f;
+            const bool plain = !e.preact && e.activation == Q6_ACT_NONE && !e.gate && !e.residual;
 #pragma unroll 1
             for (int j = 0; j < kChunk && r0 + j < p.R; j += 8) {
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = stage[(j + i) * 32 + (lane ^ ((i & 1) << 2))];
-                finish_column<T, 8>(e, p.d, r0 + j, min(8, p.R - r0 - j), p.C, c, p.gate_rows, b, f);
+                const int n = min(8, p.R - r0 - j);
+                if (plain && n == 8)
+                    finish_column<T, 8, true>(e, p.d, r0 + j, 8, p.C, c, p.gate_rows, b, f);
+                else
+                    finish_column<T, 8, false>(e, p.d, r0 + j, n, p.C, c, p.gate_rows, b, f);
             }
         }
     }

@@ -28,8 +28,11 @@ namespace q6 {
 namespace {
 
 constexpr int kTileN = 16;     // weight rows per CTA
-constexpr int kBlocks = 4;     // blocks of 32 of k per turn
-constexpr int kTurn = 32 * kBlocks;
+// Blocks of 32 of k per turn (unaligned rows load two groups for each value's
+// group), and warps per CTA at most: two such CTAs fit an SM's registers, 64 a
+// thread.
+template <bool kAligned>
+constexpr int kBlocks = kAligned ? 4 : 2;
 constexpr int kMaxWarps = 16;
 constexpr int kMost = static_cast<int>(kDenseFewRows);
 
@@ -58,31 +61,67 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight values of a row from k on, zero past K; kBytes: what the row's alignment
-// allows per load (16, 4 or 2).
-template <int kBytes>
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (kBytes == 16) {
-        if (k < K) v = __ldg(reinterpret_cast<const uint4*>(row + k));
-    } else {
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+// Eight values of a row from k on, zero past K, by element (any alignment).
+__device__ __forceinline__ uint4 load8_each(const uint16_t* row, int k, int K) {
+    uint4 v;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (kBytes == 4) {
-                if (k + 2 * i < K) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row + k + 2 * i));
-            } else {
-                const uint32_t lo = k + 2 * i < K ? __ldg(row + k + 2 * i) : 0u;
-                const uint32_t hi = k + 2 * i + 1 < K ? __ldg(row + k + 2 * i + 1) : 0u;
-                w[i] = lo | hi << 16;
-            }
-        }
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = k + 2 * i < K ? __ldg(row + k + 2 * i) : 0u;
+        const uint32_t hi = k + 2 * i + 1 < K ? __ldg(row + k + 2 * i + 1) : 0u;
+        w[i] = lo | hi << 16;
     }
     return v;
 }
 
-template <typename T, int kBytes>
-__global__ void __launch_bounds__(kMaxWarps * 32) dense_rows_kernel(const RowsParams p) {
+// The two aligned 16-byte groups around eight values of any alignment, and the
+// values shifted out of them.
+struct Around {
+    uint4 a, b;
+};
+__device__ __forceinline__ Around load_around(const uint16_t* at) {
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(15));
+    return {__ldg(p), __ldg(p + 1)};
+}
+__device__ __forceinline__ uint4 shift_out(const Around& g, uint32_t off) {
+    uint32_t w0 = g.a.x, w1 = g.a.y, w2 = g.a.z, w3 = g.a.w, w4 = g.b.x, w5 = g.b.y;
+    if (off & 8) w0 = g.a.z, w1 = g.a.w, w2 = g.b.x, w3 = g.b.y, w4 = g.b.z, w5 = g.b.w;
+    if (off & 4) w0 = w1, w1 = w2, w2 = w3, w3 = w4, w4 = w5;
+    const uint32_t bits = (off & 2) * 8;
+    return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                      __funnelshift_r(w3, w4, bits));
+}
+
+// One turn's eight-value groups of a row, k0 + 32 i + 8 t on.  Rows that are not
+// aligned 16-byte groups: where `inner` says that the groups around all of them
+// lie inside the operand (and before K), two aligned loads and a shift each; else
+// by element, which is for the ends of a sum (by element throughout, 6 x 9985 ->
+// 8729 took 93 us, 46 so).
+template <bool kAligned>
+__device__ __forceinline__ void load_turn(const uint16_t* row, int k, int K, bool inner, uint4 (&v)[kBlocks<kAligned>]) {
+    constexpr int B = kBlocks<kAligned>;
+    if constexpr (kAligned) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (k + 32 * i < K) v[i] = __ldg(reinterpret_cast<const uint4*>(row + k + 32 * i));
+        }
+    } else if (inner) {
+        Around g[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) g[i] = load_around(row + k + 32 * i);
+        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + k)) & 15;
+#pragma unroll
+        for (int i = 0; i < B; ++i) v[i] = shift_out(g[i], off);
+    } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i) v[i] = load8_each(row, k + 32 * i, K);
+    }
+}
+
+template <typename T, bool kAligned>
+__global__ void __launch_bounds__(kMaxWarps * 32, 2) dense_rows_kernel(const RowsParams p) {
+    constexpr int B = kBlocks<kAligned>, kTurn = 32 * B;
     static_assert(kMost == 8, "one MMA tile of rows of x");
     __shared__ float sums[kMaxWarps][kMost][kTileN + 1];
     pdl_launch_dependents();
@@ -96,20 +135,20 @@ __global__ void __launch_bounds__(kMaxWarps * 32) dense_rows_kernel(const RowsPa
     pdl_wait();
     float c[4] = {};
     for (int k0 = warp * kTurn; k0 < p.K; k0 += warps * kTurn) {
-        uint4 a0[kBlocks], a1[kBlocks], b[kBlocks];
+        uint4 a0[B], a1[B], b[B];
+        // the groups around a turn's values reach at most eight values beyond it
+        const bool before = k0 + kTurn + 8 <= p.K;
+        const bool inner = before && (k0 >= 8 || n0 > 0);
+        load_turn<kAligned>(w0, k0 + 8 * t, p.K, inner, a0);
+        load_turn<kAligned>(w1, k0 + 8 * t, p.K, inner, a1);
+        if (g < p.M) {
+            load_turn<kAligned>(x, k0 + 8 * t, p.K, before && k0 >= 8, b);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            const int k = k0 + 32 * i + 8 * t;
-            a0[i] = load8<kBytes>(w0, k, p.K);
-            a1[i] = load8<kBytes>(w1, k, p.K);
+            for (int i = 0; i < B; ++i) b[i] = make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            b[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (g < p.M) b[i] = load8<kBytes>(x, k0 + 32 * i + 8 * t, p.K);
-        }
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
+        for (int i = 0; i < B; ++i) {
             mma16816<T>(c, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
             mma16816<T>(c, a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
         }
@@ -141,16 +180,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32) dense_rows_kernel(const RowsPa
     }
 }
 
-template <typename T>
-cudaError_t launch_typed(const RowsParams& p, int bytes, cudaStream_t stream) {
-    // about 16 warps per SM in all, no more than the turns of one sum
-    const int64_t tiles = (p.N + kTileN - 1) / kTileN, turns = (p.K + kTurn - 1) / kTurn;
-    const int64_t want = (int64_t(device_sm_count()) * 16 + tiles - 1) / tiles;
-    const int64_t warps = std::max<int64_t>(1, std::min<int64_t>({want, turns, int64_t(kMaxWarps)}));
-    const dim3 grid(static_cast<unsigned>(tiles)), block(static_cast<unsigned>(32 * warps));
-    if (bytes == 16) return launch_pdl(dense_rows_kernel<T, 16>, grid, block, 0, stream, p);
-    if (bytes == 4) return launch_pdl(dense_rows_kernel<T, 4>, grid, block, 0, stream, p);
-    return launch_pdl(dense_rows_kernel<T, 2>, grid, block, 0, stream, p);
+template <typename T, bool kAligned>
+cudaError_t launch_typed(const RowsParams& p, cudaStream_t stream) {
+    // as many warps as let every CTA run at once, no more than the turns of one sum
+    const int64_t tiles = (p.N + kTileN - 1) / kTileN, turns = (p.K + 32 * kBlocks<kAligned> - 1) / (32 * kBlocks<kAligned>);
+    const int64_t per_sm = (tiles + device_sm_count() - 1) / device_sm_count();
+    const int64_t warps = std::max<int64_t>(
+        1, std::min<int64_t>({2 * kMaxWarps / per_sm, turns, int64_t(kMaxWarps)}));
+    return launch_pdl(dense_rows_kernel<T, kAligned>, dim3(static_cast<unsigned>(tiles)),
+                      dim3(static_cast<unsigned>(32 * warps)), 0, stream, p);
 }
 
 }  // namespace
@@ -167,14 +205,13 @@ int launch_dense_rows(const DenseProduct& a, cudaStream_t stream) {
     p.K = static_cast<int>(a.L);
     p.gate_rows = a.epi.gate ? static_cast<int>(a.epi.rows_per_gate) : p.M;
     p.epi = a.epi;
-    const auto fits = [&](int64_t bytes) {
-        const int64_t e = bytes / 2;
-        return p.K % e == 0 && p.ldw % e == 0 && p.ldx % e == 0 && reinterpret_cast<uintptr_t>(p.w) % bytes == 0 &&
-               reinterpret_cast<uintptr_t>(p.x) % bytes == 0;
-    };
-    const int bytes = fits(16) ? 16 : fits(4) ? 4 : 2;
-    const cudaError_t e = a.dtype == Q6_DTYPE_F16 ? launch_typed<__half>(p, bytes, stream)
-                                                  : launch_typed<__nv_bfloat16>(p, bytes, stream);
+    const bool aligned = p.K % 8 == 0 && p.ldw % 8 == 0 && p.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0 &&
+                         reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+    cudaError_t e;
+    if (a.dtype == Q6_DTYPE_F16)
+        e = aligned ? launch_typed<__half, true>(p, stream) : launch_typed<__half, false>(p, stream);
+    else
+        e = aligned ? launch_typed<__nv_bfloat16, true>(p, stream) : launch_typed<__nv_bfloat16, false>(p, stream);
     return e == cudaSuccess ? Q6_OK : Q6_ERR_CUDA;
 }
 
