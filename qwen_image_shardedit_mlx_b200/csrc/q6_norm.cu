@@ -177,7 +177,7 @@ int plan_grad(int64_t M, int64_t D, int64_t rows_per_vec, int dtype, bool vec, i
         plan_plain_strips(M, rows_per_vec, strip_rows, strips_per_vec);
     else
         norm_plan_strips(M, rows_per_vec,
-                         vec ? norm_detail::grad_row_lanes(kNormGrad[shape].w, kNormGrad[shape].n)
+                         vec ? norm_detail::grad_row_lanes(kNormGrad[shape].w)
                              : strided_row_lanes(kNormGradStrided[shape].w),
                          strip_rows, strips_per_vec);
     return shape;

@@ -327,18 +327,17 @@ __device__ __forceinline__ void finish_columns(const NormParams& p, const C& at,
 // shuffles, barrier and sums left the SM idle.
 //   In B: with u = dy rstd and t = x - mean,
 //   dx = u w + t k + c,  k = -rstd^2 mean_D(a xh),  c = -rstd mean_D(a);  dweight += u t.
-// Row lanes: about 768 threads (576 with two groups of columns per thread).
-constexpr int grad_row_lanes(int cw, int n) {
-    const int threads = n == 1 ? 768 : 576;
-    return threads / (32 * cw) < 1 ? 1 : threads / (32 * cw);
-}
+// Row lanes: about 384 threads.  Fewer threads mean smaller tiles, so more of
+// them in flight: with 576, two stages of 72 KB, a tile's copy had half a tile's
+// time to land (65536 x 1024 fp16 110 us, 80 so; 256 threads 96).
+constexpr int grad_row_lanes(int cw) { return 12 / cw < 1 ? 1 : 12 / cw; }
 constexpr int kGradSmem = 208 * 1024;
-constexpr int kGradMaxStages = 4;
+constexpr int kGradMaxStages = 8;
 
 template <typename T, typename V, Layout kLay, int CW, int N, int M>
-__global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW, N), 1)
+__global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
     norm_grad_kernel(const NormParams p, V* dweight, V* dbias, const int stages) {
-    constexpr int G = 16 / sizeof(T), P = G / 2, RL = grad_row_lanes(CW, N), TR = RL * M;
+    constexpr int G = 16 / sizeof(T), P = G / 2, RL = grad_row_lanes(CW), TR = RL * M;
     constexpr int AP = CW >= M ? CW / M : 1, AR = CW >= M ? 1 : M / CW;  // warps per row and rows per warp in phase A
     static_assert((CW >= M ? CW % M : M % CW) == 0 && kLay != kStrided, "phase A");
     __shared__ __align__(16) float2 parts[2][TR][AP];
@@ -626,8 +625,8 @@ struct NormShape {
     int w, n, m;
 };
 constexpr NormShape kNormForward[] = {{1, 1}, {1, 2}, {1, 4}, {2, 4}, {3, 4}, {4, 4}, {6, 4}, {8, 4}, {12, 4}, {16, 4}, {32, 4}};
-constexpr NormShape kNormGrad[] = {{1, 1, 2}, {1, 2, 2}, {2, 2, 2},  {3, 2, 1},  {4, 2, 2},  {6, 2, 2},
-                                   {8, 2, 2}, {12, 2, 2}, {16, 2, 2}, {24, 2, 1}, {32, 2, 1}};
+constexpr NormShape kNormGrad[] = {{1, 1, 4}, {1, 2, 2}, {2, 2, 2},  {3, 2, 3},  {4, 2, 2}, {6, 2, 2},
+                                   {8, 2, 2}, {12, 2, 2}, {16, 2, 2}, {12, 4, 1}, {16, 4, 1}};
 constexpr NormShape kNormGradStrided[] = {{1, 1, 1}, {1, 2, 1}, {2, 2, 1}, {4, 2, 1}, {8, 2, 1}, {16, 2, 1}, {16, 4, 1}};
 constexpr int strided_row_lanes(int w) { return w < 16 ? 16 / w : 1; }
 
@@ -688,7 +687,7 @@ bool norm_opt_in(void (*kernel)(A...), int bytes, std::atomic<bool> (&done)[kMax
 template <typename T, typename V, norm_detail::Layout kLay, int W, int N, int M>
 int launch_norm_grad(const NormParams& p, V* dweight, V* dbias, cudaStream_t stream) {
     using namespace norm_detail;
-    constexpr int lanes = grad_row_lanes(W, N), tile_rows = lanes * M;
+    constexpr int lanes = grad_row_lanes(W), tile_rows = lanes * M;
     auto* kernel = norm_grad_kernel<T, V, kLay, W, N, M>;
     static std::atomic<bool> done[kMaxDevices];
     if (!norm_opt_in(kernel, kGradSmem, done)) return Q6_ERR_CUDA;
