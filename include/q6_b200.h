@@ -305,7 +305,8 @@ enum q6_activation {
  *   gate: row m takes vector m / rows_per_gate of gate [.., N] (ldg elements apart);
  *   rows_per_gate divides M (M: one vector for all rows).
  * bias, gate, residual may be null.  preact (nullable, [M, N] dense, element type
- * preact_dtype: dtype or F32) receives z, which q6_dense_linear_grad reads.
+ * preact_dtype: F16, held at the largest fp16 value, or F32) receives z, which
+ * q6_dense_linear_grad reads.
  * dtype: BF16 or F16.
  * y may alias residual (same layout), nothing else may overlap an output.
  * workspace: at least q6_dense_linear_workspace_bytes, 256-byte aligned.

@@ -372,7 +372,7 @@ int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     const int st = check_common(M, N, K, dtype, activation, gate, ldg, rows_per_gate);
     if (st != Q6_OK) return st;
     if (!x || !w || !y) return Q6_ERR_INVALID_ARGUMENT;
-    if (preact && preact_dtype != dtype && preact_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
+    if (preact && preact_dtype != Q6_DTYPE_F16 && preact_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
     if (!stride_ok(ldx, K, M) || !stride_ok(ldw, K, N) || (residual && !stride_ok(ldr, N, M)))
         return Q6_ERR_INVALID_ARGUMENT;
     for (const void* t : {x, w, bias, gate, residual, static_cast<const void*>(y), static_cast<const void*>(preact)})
@@ -439,7 +439,7 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
     if (st != Q6_OK) return st;
     if (!dy || (dw && !x) || (dx && !w)) return Q6_ERR_INVALID_ARGUMENT;
     if (!preact && (activation != Q6_ACT_NONE || dgate)) return Q6_ERR_INVALID_ARGUMENT;
-    if (preact && preact_dtype != dtype && preact_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
+    if (preact && preact_dtype != Q6_DTYPE_F16 && preact_dtype != Q6_DTYPE_F32) return Q6_ERR_UNSUPPORTED;
     if (dgate && !gate) return Q6_ERR_INVALID_ARGUMENT;
     if (!stride_ok(ldy, N, M) || (dw && !stride_ok(ldx, K, M)) || (dx && !stride_ok(ldw, K, N)))
         return Q6_ERR_INVALID_ARGUMENT;
@@ -483,7 +483,7 @@ int q6_dense_linear_grad(const void* dy, int64_t ldy, const void* x, int64_t ldx
         int e;
         if (dtype == Q6_DTYPE_BF16)
             e = f32 ? run_dz_act<__nv_bfloat16, float>(z, activation, M, dbias, dgate, stream)
-                    : run_dz_act<__nv_bfloat16, __nv_bfloat16>(z, activation, M, dbias, dgate, stream);
+                    : run_dz_act<__nv_bfloat16, __half>(z, activation, M, dbias, dgate, stream);
         else
             e = f32 ? run_dz_act<__half, float>(z, activation, M, dbias, dgate, stream)
                     : run_dz_act<__half, __half>(z, activation, M, dbias, dgate, stream);

@@ -50,16 +50,28 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 0 or 1 to the last bit), so that no product of infinities with zeros can arise.
 __device__ __forceinline__ float act_sigmoid(float z, int act, float& t) {
     if (act == Q6_ACT_GELU_TANH) {
-        t = fminf(z * z, 400.0f);
-        return rcp_f(1.0f + ex2_f(z * fmaf(t, -kLog2e * kGelu2K * kGeluC, -kLog2e * kGelu2K)));
+        t = fminf(__fmul_rn(z, z), 400.0f);
+        return rcp_f(__fadd_rn(1.0f, ex2_f(__fmul_rn(z, fmaf(t, -kLog2e * kGelu2K * kGeluC, -kLog2e * kGelu2K)))));
     }
-    return rcp_f(1.0f + ex2_f(-kLog2e * z));
+    return rcp_f(__fadd_rn(1.0f, ex2_f(__fmul_rn(-kLog2e, z))));
 }
 
+// The epilogue's steps are written with explicit roundings (here and below): left
+// to the compiler, a product and a sum may or may not become one operation, by
+// what else a kernel writes, and a forward pass with and without gradients would
+// differ in its last bits.
 __device__ __forceinline__ float act_f(float z, int act) {
     if (act == Q6_ACT_NONE) return z;
     float t;
-    return z * act_sigmoid(z, act, t);
+    return __fmul_rn(z, act_sigmoid(z, act, t));
+}
+
+// A pre-activation as the backward pass reads it: fp16 whatever the operands' type
+// (three more bits than bf16 for the values it has: its rounding disappears
+// behind that of dz), held at the largest fp16 value, beyond which every
+// activation's slope is 0 or 1.  NaN stays NaN.
+__device__ __forceinline__ __half preact_half(float z) {
+    return __float2half_rn(z > 65504.0f ? 65504.0f : z < -65504.0f ? -65504.0f : z);
 }
 
 // 16-byte (or smaller) read-only loads: free to move across stores.

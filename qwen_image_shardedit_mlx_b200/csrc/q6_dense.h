@@ -17,7 +17,7 @@ struct DenseEpilogue {
     int64_t ldg = 0, rows_per_gate = 1;
     const void* residual = nullptr;  // [R, C], row stride ldr
     int64_t ldr = 0;
-    void* preact = nullptr;          // [R, C] dense, in dtype or (preact_f32) fp32
+    void* preact = nullptr;          // [R, C] dense, fp16 (preact_half) or (preact_f32) fp32
     bool preact_f32 = false;
     int activation = Q6_ACT_NONE;
 };

@@ -164,7 +164,7 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
                                         const Eight<T>& bias, const Eight<T>& residual, float (&v)[8]) {
     if (e.bias) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += to_f(bias.v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], to_f(bias.v[i]));
     }
     const int64_t at = r * C + c;
     if (e.preact) {
@@ -173,10 +173,10 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
             z[0] = make_float4(v[0], v[1], v[2], v[3]);
             z[1] = make_float4(v[4], v[5], v[6], v[7]);
         } else {
-            Eight<T> z;
+            Eight<__half> z;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z.v[i] = from_f<T>(v[i]);
-            *reinterpret_cast<Eight<T>*>(static_cast<T*>(e.preact) + at) = z;
+            for (int i = 0; i < 8; ++i) z.v[i] = preact_half(v[i]);
+            *reinterpret_cast<Eight<__half>*>(static_cast<__half*>(e.preact) + at) = z;
         }
     }
     if (e.activation == Q6_ACT_GELU_TANH) {
@@ -189,11 +189,11 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
     if (e.gate) {
         const Eight<T> g = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(e.gate) + gate_row * e.ldg + c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= to_f(g.v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], to_f(g.v[i]));
     }
     if (e.residual) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += to_f(residual.v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], to_f(residual.v[i]));
     }
     Eight<T> y;
 #pragma unroll
@@ -210,7 +210,7 @@ __device__ __forceinline__ void finish_column(const DenseEpilogue& e, void* d, i
     if constexpr (kPlain) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i, y += C)
-            if (i < n) *y = from_f<T>(v[i] + bias);
+            if (i < n) *y = from_f<T>(__fadd_rn(v[i], bias));
     } else {
         T res[kRows], gate[kRows];
 #pragma unroll
@@ -224,16 +224,16 @@ __device__ __forceinline__ void finish_column(const DenseEpilogue& e, void* d, i
 #pragma unroll
         for (int i = 0; i < kRows; ++i, at += C, y += C) {
             if (i < n) {
-                float t = v[i] + bias;
+                float t = __fadd_rn(v[i], bias);
                 if (e.preact) {
                     if (e.preact_f32)
                         static_cast<float*>(e.preact)[at] = t;
                     else
-                        static_cast<T*>(e.preact)[at] = from_f<T>(t);
+                        static_cast<__half*>(e.preact)[at] = preact_half(t);
                 }
                 t = act_f(t, e.activation);
-                if (e.gate) t *= to_f(gate[i]);
-                if (e.residual) t += to_f(res[i]);
+                if (e.gate) t = __fmul_rn(t, to_f(gate[i]));
+                if (e.residual) t = __fadd_rn(t, to_f(res[i]));
                 *y = from_f<T>(t);
             }
         }

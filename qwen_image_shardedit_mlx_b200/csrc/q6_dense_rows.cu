@@ -165,17 +165,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) dense_rows_kernel(const Row
         if (n >= p.N) continue;
         float v = 0.0f;
         for (int k = 0; k < warps; ++k) v += sums[k][m][i % kTileN];
-        if (e.bias) v += to_f(static_cast<const T*>(e.bias)[n]);
+        if (e.bias) v = __fadd_rn(v, to_f(static_cast<const T*>(e.bias)[n]));
         const int64_t at = int64_t(m) * p.N + n;
         if (e.preact) {
             if (e.preact_f32)
                 static_cast<float*>(e.preact)[at] = v;
             else
-                static_cast<T*>(e.preact)[at] = from_f<T>(v);
+                static_cast<__half*>(e.preact)[at] = preact_half(v);
         }
         v = act_f(v, e.activation);
-        if (e.gate) v *= to_f(static_cast<const T*>(e.gate)[m / p.gate_rows * e.ldg + n]);
-        if (e.residual) v += to_f(static_cast<const T*>(e.residual)[m * e.ldr + n]);
+        if (e.gate) v = __fmul_rn(v, to_f(static_cast<const T*>(e.gate)[m / p.gate_rows * e.ldg + n]));
+        if (e.residual) v = __fadd_rn(v, to_f(static_cast<const T*>(e.residual)[m * e.ldr + n]));
         static_cast<T*>(p.y)[at] = from_f<T>(v);
     }
 }

@@ -156,8 +156,8 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
     const int64_t n = w.size(0), k = w.size(1), m = x.numel() / k;
     const auto shape = with_last(x, n);
     Tensor y = like(x, shape, x.scalar_type());
-    // the gate's gradient sums act(z) itself: rounded to 16 bits, z would cost it as much as its own rounding
-    const auto zt = gate.defined() ? at::kFloat : x.scalar_type();
+    // the gate's gradient sums act(z) itself: rounded to 16 bits, z could cost it as much as its own rounding
+    const auto zt = gate.defined() ? at::kFloat : at::kHalf;
     Tensor z = save_preact ? like(x, shape, zt) : Tensor();
     if (m == 0) return {y, z};
     const Rows rx = rows_of(x, k), rw = rows_of(w, k), rr = rows_of(residual, n), rg = rows_of(gate, n);
@@ -197,7 +197,8 @@ LinearGrads linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, 
     const std::pair<const char*, const Tensor*> named[] = {
         {"x", &x}, {"weight", &w}, {"preact", &preact}, {"gate", &gate}};
     for (const auto& [name, t] : named)
-        TORCH_CHECK_VALUE(!t->defined() || t->scalar_type() == dt || (t == &preact && t->scalar_type() == at::kFloat),
+        TORCH_CHECK_VALUE(!t->defined() || (t == &preact ? t->scalar_type() == at::kFloat || t->scalar_type() == at::kHalf
+                                                         : t->scalar_type() == dt),
                           name, " is ", t->scalar_type(), ", dy is ", dt);
     const int64_t m = dy.numel() / n;
     const int64_t rows_per_gate = gate.defined() ? sample_rows("gate", gate.sizes(), dy, n) : m;
@@ -220,7 +221,7 @@ LinearGrads linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, 
                                                               pack);
     const Tensor ws = workspace(bytes, dy);
     check(q6_dense_linear_grad(ptr(ry.t), ry.ld, ptr(rx.t), rx.ld, ptr(rw.t), rw.ld, ptr(z),
-                               dtype_code(z.defined() ? z.scalar_type() : dt), ptr(rg.t), rg.ld, rows_per_gate,
+                               dtype_code(z.defined() ? z.scalar_type() : at::kHalf), ptr(rg.t), rg.ld, rows_per_gate,
                                mutable_ptr(g.x), mutable_ptr(g.weight), mutable_ptr(g.bias), mutable_ptr(g.gate), m, n,
                                k, dtype_code(dt), activation, mutable_ptr(ws), bytes, stream_of(dy)),
           "q6_dense_linear_grad");

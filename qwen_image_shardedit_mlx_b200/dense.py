@@ -105,8 +105,9 @@ def dense_linear_forward(
     save_preact: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(y, preact): ``dense_linear`` without autograd.  With ``save_preact`` the
-    second value is ``x @ W^T + bias`` (in x's dtype, or in fp32 when a gate is
-    given), which ``dense_linear_backward`` takes; else None."""
+    second value is ``x @ W^T + bias`` for ``dense_linear_backward``, in fp16
+    (whatever x's dtype, held at the largest fp16 value, beyond which the slope of
+    every activation is 0 or 1), or in fp32 when a gate is given; else None."""
 
     return _native().dense_linear_forward(x, weight, bias, _activation(activation), residual, gate, save_preact)
 

@@ -46,8 +46,9 @@ def test_linear_refuses(kw, match):
     (dict(x=None), "needs x"),
     (dict(weight=None), "needs weight"),
     (dict(activation="silu"), "preact"),
-    (dict(outputs=("gate",), preact=t(4, 6)), "needs gate"),
-    (dict(preact=t(4, 5)), "preact must be"),
+    (dict(preact=t(4, 6)), "preact is"),
+    (dict(outputs=("gate",), preact=t(4, 6, dtype=torch.float16)), "needs gate"),
+    (dict(preact=t(4, 5, dtype=torch.float16)), "preact must be"),
     (dict(x=t(5, 8)), "does not match"),
     (dict(weight=t(7, 8)), "does not match"),
     (dict(x=t(4, 8, dtype=torch.float16)), "x is"),
@@ -104,7 +105,7 @@ def test_c_entries_refuse_before_the_device():
     assert linear(ldx=63) == inv and linear(ldw=60) == inv and linear(res=256, ldr=31) == inv
     assert linear(rpg=3) == inv and linear(rpg=0) == inv and linear(rpg=2, gate=256, ldg=16) == inv
     assert linear(act=3) == inv and linear(act=-1) == inv
-    assert linear(dtype=2) == uns and linear(pre=256, pdt=1) == uns and linear(pre=258, pdt=2) == al
+    assert linear(dtype=2) == uns and linear(pre=256, pdt=0) == uns and linear(pre=258, pdt=2) == al
     assert linear(x=257) == al and linear(y=255) == al and linear(ws=128, wsb=1 << 30) == al
     assert linear(M=40, rpg=40, x=258) == wsp  # an operand off its 16 bytes is copied: the workspace must hold it
     assert lib.q6_dense_linear_workspace_bytes(40, 32, 64, _lib.Q6_PACK_X) >= 40 * 64 * 2
