@@ -64,6 +64,7 @@ enum q6_error_site {
     Q6_SITE_GEMM_MIN = 1,       /* 1..12: GEMM, GEMV and few-row MMA pipeline barriers */
     Q6_SITE_GEMM_MAX = 12,
     Q6_SITE_PEER_BARRIER = 13,  /* q6_sp_barrier: a peer's flag did not arrive in time */
+    Q6_SITE_NORM_RING = 40,     /* q6_layer_norm_grad: a tile's copy did not arrive in time */
     Q6_SITE_SELFTEST = 64       /* q6_selftest_bounded_wait */
 };
 

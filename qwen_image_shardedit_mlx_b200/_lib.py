@@ -28,6 +28,7 @@ Q6_EPI_GELU_PRECISE = 2
 Q6_LORA_B_NMAJOR = 4
 
 Q6_SITE_PEER_BARRIER = 13
+Q6_SITE_NORM_RING = 40
 Q6_SITE_SELFTEST = 64
 
 Q6_DTYPE_BF16 = 0

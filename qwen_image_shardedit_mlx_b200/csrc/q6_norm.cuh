@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
     for (int i = 0; i < tiles; ++i) {
         const int flip = i & 1, n = min(TR, rows - i * TR);
         const uint8_t* tile = smem + static_cast<size_t>(s) * tile_bytes;
-        mbar_wait(smem_u32(full + s), phase, &abort_word, 40);
+        mbar_wait(smem_u32(full + s), phase, &abort_word, Q6_SITE_NORM_RING);
         // ---------------------------------------------------------------- phase A
         float mean[AR], rstd[AR];
 #pragma unroll
