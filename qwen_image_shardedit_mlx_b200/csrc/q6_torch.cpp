@@ -79,7 +79,7 @@ int64_t sample_rows(const char* name, at::IntArrayRef v, const Tensor& x, int64_
     TORCH_CHECK_VALUE(ok, name, " must be [", width, "] or [samples, ", width, "], got ", v);
     if (v[0] == 1) return m;
     TORCH_CHECK_VALUE(x.dim() >= 2 && v[0] == x.size(0), name, " ", v, " does not match the samples of x ", x.sizes());
-    return m / v[0];
+    return m ? m / v[0] : 0;  // without rows there may be no vectors either
 }
 
 void check_devices(const Tensor& x, std::initializer_list<const Tensor*> others) {

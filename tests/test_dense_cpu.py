@@ -187,3 +187,15 @@ def test_reference_norm_gradients_against_differences():
         lo[i], hi[i] = arg - h * v, arg + h * v
         diff = (loss(*hi) - loss(*lo)) / (2 * h)
         assert abs(diff - (got[i].v.reshape(v.shape) * v).sum()) < 1e-7
+
+
+def test_no_samples_with_a_vector_each():
+    """A batch of no samples carries no vectors either: checked like any other call."""
+    with pytest.raises(RuntimeError, match="CUDA"):
+        dense.dense_linear(t(0, 4, 8), t(6, 8), gate=t(0, 6))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        dense.dense_linear_backward(t(0, 4, 6), t(0, 4, 8), t(6, 8), gate=t(0, 6), outputs=("x",))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        dense.layer_norm_modulate(t(0, 4, 8), t(0, 8), t(0, 8))
+    with pytest.raises(ValueError, match="samples"):
+        dense.dense_linear(t(2, 4, 8), t(6, 8), gate=t(0, 6))

@@ -47,7 +47,7 @@ def make_linear(samples, rows, k, n, dtype, *, bias=True, gate=True, residual=Tr
     return x, w, b, g, r, dy
 
 
-def check_linear(x, w, b, g, r, dy, activation, *, strict=True):
+def check_linear(x, w, b, g, r, dy, activation):
     """Forward and every gradient of one call against the bounds."""
     dtype, (n, k) = x.dtype, w.shape
     m = x.numel() // k
@@ -202,6 +202,18 @@ def test_linear_empty_rows():
     y.sum().backward()
     assert torch.equal(w.grad, torch.zeros_like(w)) and torch.equal(b.grad, torch.zeros_like(b))
     assert x.grad.shape == x.shape
+
+
+def test_no_samples_with_a_vector_each():
+    x = torch.empty((0, 5, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    w = rand((24, 16), torch.bfloat16, 1).requires_grad_(True)
+    g = torch.empty((0, 24), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    scale = torch.empty((0, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    y = dense.dense_linear(dense.layer_norm_modulate(x, scale, scale), w, activation="silu", gate=g)
+    assert y.shape == (0, 5, 24)
+    y.sum().backward()
+    assert x.grad.shape == x.shape and g.grad.shape == g.shape and scale.grad.shape == scale.shape
+    assert torch.equal(w.grad, torch.zeros_like(w))
 
 
 def test_linear_partial_gradients_equal_the_whole():
