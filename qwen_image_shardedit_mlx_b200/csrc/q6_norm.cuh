@@ -7,12 +7,12 @@
 // pass over registers); one rounding at each output.
 //
 // Both directions are bound by HBM: the forward reads x and writes y, the
-// backward reads x and dy and writes dx, once each.  A row is held in the
-// registers of one thread group of W warps, so nothing is read twice.  In the backward a
-// thread keeps the same columns for every row it sees, so the weight's and
-// bias's gradients accumulate in registers over a strip of rows; a CTA adds
-// its thread groups in order, and a second kernel adds the strips' sums in
-// order.  No atomics: equal calls give equal bits.
+// backward reads x and dy and writes dx, once each: the forward holds a row in
+// the registers of one thread group of W warps, the backward a tile of rows in
+// shared memory.  In the backward a thread keeps the same columns for every row
+// it sees, so the weight's and bias's gradients accumulate in registers over a
+// strip of rows; a CTA adds its thread groups in order, and a second kernel adds
+// the strips' sums in order.  No atomics: equal calls give equal bits.
 //
 // Each thread holds N groups of G elements (16 bytes).  Where D, strides and
 // addresses allow it a group is one 16-byte access; else its G elements lie a

@@ -245,6 +245,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         refuse_second_order("dense_linear");
         const Tensor& dy = dys[0];
         if (!dy.defined()) return variable_list(6);
+        refuse_capture(dy, "dense_linear");
         const auto saved = ctx->get_saved_variables();
         // edges are numbered over the tensors that were given
         const int64_t present = ctx->saved_data["present"].toInt();
@@ -383,6 +384,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         refuse_second_order("layer_norm");
         const Tensor& dy = dys[0];
         if (!dy.defined()) return variable_list(5);
+        refuse_capture(dy, (ctx->saved_data["flags"].toInt() & Q6_NORM_ONE_PLUS) ? "layer_norm_modulate" : "layer_norm");
         const auto saved = ctx->get_saved_variables();
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const int64_t present = ctx->saved_data["present"].toInt();

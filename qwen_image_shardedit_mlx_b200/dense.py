@@ -12,8 +12,9 @@ The trainable twins of what the q6 block computes around its packed weights:
 Both differentiate through ``torch.autograd`` and have functional forms
 (``*_forward`` / ``*_backward``) that launch the same kernels without it.  The
 functional forms may be captured in a CUDA graph.  A differentiable call under
-capture is refused: its backward pass would run on the streams that autograd
-recorded for the leaves, outside the capture.
+capture, and the backward pass of an earlier one, are refused: autograd would
+run parts of it on the streams that it recorded for the leaves, outside the
+capture.
 
 Tensors must live on one CUDA device; kernels are ordered on its current
 stream, nothing synchronises, and equal calls give equal bits.  The checks, the

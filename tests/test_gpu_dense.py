@@ -310,6 +310,27 @@ def test_linear_capture_with_gradients_is_refused():
     assert torch.equal(y, dense.dense_linear(x, w.detach(), b))
 
 
+def test_captured_backward_of_an_eager_call_is_refused():
+    x, w, b, _, _, _ = make_linear(1, 12, 16, 16, torch.bfloat16)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for name, f in (("dense_linear_backward", lambda leaf: dense.dense_linear(x, w, leaf)),
+                        ("layer_norm_backward", lambda leaf: dense.layer_norm(x, None, leaf))):
+            leaf = b.detach().requires_grad_(True)
+            y = f(leaf)
+            dy = torch.ones_like(y)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                with pytest.raises(RuntimeError, match=name):
+                    torch.autograd.grad(y, leaf, dy, retain_graph=True)
+                z = dy + 1
+            graph.replay()
+            (grad,) = torch.autograd.grad(y, leaf, dy)  # outside a capture as ever
+            assert torch.equal(grad, torch.full_like(b, 12.0)) and torch.equal(z, dy + 1)
+    torch.cuda.current_stream().wait_stream(stream)
+
+
 def test_linear_residual_rows_around_the_output_are_left_alone():
     x, w, b, _, _, _ = make_linear(1, 37, 40, 56, torch.bfloat16, gate=False)
     guard = torch.full((3, 37, 56), 7.0, dtype=torch.bfloat16, device="cuda")
