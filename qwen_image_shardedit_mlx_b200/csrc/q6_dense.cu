@@ -300,10 +300,10 @@ struct Carver {
 
 // The few-row kernel reads its operands where they are; Q6_DENSE_PLAN (a plan of
 // the tensor-core path) turns it off.
-bool few_rows(int64_t M) { return M <= kDenseFewRows && !std::getenv("Q6_DENSE_PLAN"); }
+bool few_rows(int64_t M, int64_t N, int64_t K) { return dense_few_rows(M, N, K) && !std::getenv("Q6_DENSE_PLAN"); }
 
 size_t forward_bytes(int64_t M, int64_t N, int64_t K, int pack) {
-    if (few_rows(M)) return 0;
+    if (few_rows(M, N, K)) return 0;
     size_t b = round_up(dense_product_workspace_bytes(M, N, K, false, false));
     if (pack & Q6_PACK_X) b += round_up(size_t(M) * pad8(K) * 2);
     if (pack & Q6_PACK_W) b += round_up(size_t(N) * pad8(K) * 2);
@@ -401,7 +401,7 @@ int q6_dense_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     a.epi.preact = preact;
     a.epi.preact_f32 = preact_dtype == Q6_DTYPE_F32;
     a.epi.activation = activation;
-    const bool rows = few_rows(M);
+    const bool rows = few_rows(M, N, K);
     Carver ws{static_cast<char*>(workspace)};
     if (!rows) {
         a.workspace_bytes = dense_product_workspace_bytes(M, N, K, false, false);

@@ -40,9 +40,9 @@ struct DenseProduct {
     size_t workspace_bytes = 0;
 };
 
-// Up to kDenseFewRows rows of Q, both operands with the sum contiguous, any
-// alignment, no workspace (q6_dense_rows.cu).
-constexpr int64_t kDenseFewRows = 8;
+// A few rows of Q (R <= 16), both operands with the sum contiguous, any alignment,
+// no workspace (q6_dense_rows.cu).
+bool dense_few_rows(int64_t R, int64_t C, int64_t L);  // where it is the faster path
 int launch_dense_rows(const DenseProduct& a, cudaStream_t stream);
 
 int launch_dense_product(const DenseProduct& a, cudaStream_t stream);

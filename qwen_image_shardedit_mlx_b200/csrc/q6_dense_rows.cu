@@ -1,20 +1,20 @@
-// Dense linear for a few rows (1 to 8): bound by reading the weight once.
+// Dense linear for a few rows (1 to 16): bound by reading the weight once.
 //
 //   y[m, n] = epilogue(sum_k x[m, k] W[n, k])
 //
-// A CTA takes 16 rows of W; its warps share the sum, 128 of k at a time.  The
-// products run on warp-level MMAs (m16n8k16) with the weight rows as the A operand
-// and the rows of x as B, straight from global memory: within a block of 32 of k
+// A CTA takes 16 rows of W; its warps share the sum, 128 of k at a time (64 from
+// nine rows of x on, which are two MMA tiles).  The products run on warp-level
+// MMAs (m16n8k16) with the weight rows as the A operand and the rows of x as B,
+// straight from global memory: within a block of 32 of k
 // lane t of a row holds eight neighbouring values (one 16-byte load), and since
 // both operands number the sum's terms the same way, the MMA's own order of them
 // does not matter.  So the weight passes through no shared memory and no
 // shuffles; eight 16-byte loads of it per lane are in flight per turn.  The warps'
 // partial sums meet in shared memory and are added in order.
 //
-// bf16, one row: 3072 -> 18432 20.0 us (5.7 TB/s), 3072 -> 3072 6.2 us, 12288 -> 3072
-// 16.6 us; the tcgen05 path, which needs a second kernel for its split sums, takes
-// 20.9, 9.2 and 17.8.  At sixteen rows x is read as often as the weight and the
-// tcgen05 path wins (3072 -> 3072 9.4 against 11.4 us), so this one ends at eight.
+// bf16, one row: 3072 -> 18432 19.5 us (5.8 TB/s), 3072 -> 3072 6.3 us, 12288 -> 3072
+// 15.1 us; the tcgen05 path, which needs a second kernel for its split sums, takes
+// 20.9, 9.2 and 17.8.  (dense_few_rows has the figures of sixteen rows.)
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -31,10 +31,10 @@ constexpr int kTileN = 16;     // weight rows per CTA
 // Blocks of 32 of k per turn (unaligned rows load two groups for each value's
 // group), and warps per CTA at most: two such CTAs fit an SM's registers, 64 a
 // thread.
-template <bool kAligned>
-constexpr int kBlocks = kAligned ? 4 : 2;
+template <bool kAligned, int MT>
+constexpr int kBlocks = (kAligned ? 4 : 2) / MT;
 constexpr int kMaxWarps = 16;
-constexpr int kMost = static_cast<int>(kDenseFewRows);
+constexpr int kTileM = 8;  // rows of x per MMA; MT such tiles
 
 struct RowsParams {
     const void* x;
@@ -97,9 +97,8 @@ __device__ __forceinline__ uint4 shift_out(const Around& g, uint32_t off) {
 // lie inside the operand (and before K), two aligned loads and a shift each; else
 // by element, which is for the ends of a sum (by element throughout, 6 x 9985 ->
 // 8729 took 93 us, 46 so).
-template <bool kAligned>
-__device__ __forceinline__ void load_turn(const uint16_t* row, int k, int K, bool inner, uint4 (&v)[kBlocks<kAligned>]) {
-    constexpr int B = kBlocks<kAligned>;
+template <bool kAligned, int B>
+__device__ __forceinline__ void load_turn(const uint16_t* row, int k, int K, bool inner, uint4 (&v)[B]) {
     if constexpr (kAligned) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
@@ -119,11 +118,10 @@ __device__ __forceinline__ void load_turn(const uint16_t* row, int k, int K, boo
     }
 }
 
-template <typename T, bool kAligned>
+template <typename T, bool kAligned, int MT>
 __global__ void __launch_bounds__(kMaxWarps * 32, 2) dense_rows_kernel(const RowsParams p) {
-    constexpr int B = kBlocks<kAligned>, kTurn = 32 * B;
-    static_assert(kMost == 8, "one MMA tile of rows of x");
-    __shared__ float sums[kMaxWarps][kMost][kTileN + 1];
+    constexpr int B = kBlocks<kAligned, MT>, kTurn = 32 * B;
+    __shared__ float sums[kMaxWarps][MT * kTileM][kTileN + 1];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -133,31 +131,40 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) dense_rows_kernel(const Row
     const uint16_t* w1 = static_cast<const uint16_t*>(p.w) + int64_t(min(n0 + g + 8, p.N - 1)) * p.ldw;
     const uint16_t* x = static_cast<const uint16_t*>(p.x) + g * p.ldx;
     pdl_wait();
-    float c[4] = {};
+    float c[MT][4] = {};
     for (int k0 = warp * kTurn; k0 < p.K; k0 += warps * kTurn) {
-        uint4 a0[B], a1[B], b[B];
+        uint4 a0[B], a1[B], b[MT][B];
         // the groups around a turn's values reach at most eight values beyond it
         const bool before = k0 + kTurn + 8 <= p.K;
         const bool inner = before && (k0 >= 8 || n0 > 0);
         load_turn<kAligned>(w0, k0 + 8 * t, p.K, inner, a0);
         load_turn<kAligned>(w1, k0 + 8 * t, p.K, inner, a1);
-        if (g < p.M) {
-            load_turn<kAligned>(x, k0 + 8 * t, p.K, before && k0 >= 8, b);
-        } else {
 #pragma unroll
-            for (int i = 0; i < B; ++i) b[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int h = 0; h < MT; ++h) {
+            if (g + h * kTileM < p.M) {
+                load_turn<kAligned>(x + h * kTileM * p.ldx, k0 + 8 * t, p.K, before && k0 >= 8, b[h]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < B; ++i) b[h][i] = make_uint4(0u, 0u, 0u, 0u);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            mma16816<T>(c, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
-            mma16816<T>(c, a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
-        }
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int h = 0; h < MT; ++h) {
+                mma16816<T>(c[h], a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[h][i].x, b[h][i].y);
+                mma16816<T>(c[h], a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[h][i].z, b[h][i].w);
+            }
     }
-    // c: weight rows g and g + 8, rows 2 t and 2 t + 1 of x
-    sums[warp][2 * t][g] = c[0];
-    sums[warp][2 * t + 1][g] = c[1];
-    sums[warp][2 * t][g + 8] = c[2];
-    sums[warp][2 * t + 1][g + 8] = c[3];
+    // c: weight rows g and g + 8, rows 2 t and 2 t + 1 of a tile of x
+#pragma unroll
+    for (int h = 0; h < MT; ++h) {
+        float(*to)[kTileN + 1] = sums[warp] + h * kTileM + 2 * t;
+        to[0][g] = c[h][0];
+        to[1][g] = c[h][1];
+        to[0][g + 8] = c[h][2];
+        to[1][g + 8] = c[h][3];
+    }
     __syncthreads();
     const DenseEpilogue& e = p.epi;
     for (int i = threadIdx.x; i < p.M * kTileN; i += blockDim.x) {
@@ -180,18 +187,34 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) dense_rows_kernel(const Row
     }
 }
 
-template <typename T, bool kAligned>
-cudaError_t launch_typed(const RowsParams& p, cudaStream_t stream) {
+template <typename T, bool kAligned, int MT>
+cudaError_t launch_tiles(const RowsParams& p, cudaStream_t stream) {
+    constexpr int kTurn = 32 * kBlocks<kAligned, MT>;
     // as many warps as let every CTA run at once, no more than the turns of one sum
-    const int64_t tiles = (p.N + kTileN - 1) / kTileN, turns = (p.K + 32 * kBlocks<kAligned> - 1) / (32 * kBlocks<kAligned>);
+    const int64_t tiles = (p.N + kTileN - 1) / kTileN, turns = (p.K + kTurn - 1) / kTurn;
     const int64_t per_sm = (tiles + device_sm_count() - 1) / device_sm_count();
     const int64_t warps = std::max<int64_t>(
         1, std::min<int64_t>({2 * kMaxWarps / per_sm, turns, int64_t(kMaxWarps)}));
-    return launch_pdl(dense_rows_kernel<T, kAligned>, dim3(static_cast<unsigned>(tiles)),
+    return launch_pdl(dense_rows_kernel<T, kAligned, MT>, dim3(static_cast<unsigned>(tiles)),
                       dim3(static_cast<unsigned>(32 * warps)), 0, stream, p);
 }
 
+template <typename T, bool kAligned>
+cudaError_t launch_typed(const RowsParams& p, cudaStream_t stream) {
+    return p.M <= kTileM ? launch_tiles<T, kAligned, 1>(p, stream) : launch_tiles<T, kAligned, 2>(p, stream);
+}
+
 }  // namespace
+
+// Up to eight rows always.  To sixteen, x is as large as a CTA's part of the
+// weight, and an SM takes in both: the tcgen05 path, which reads x once per 128
+// rows of W, wins where the sum is long or the weight large.  Sixteen rows of bf16,
+// here against there: 768 -> 768 2.8 / 5.7 us, 3072 -> 3072 7.9 / 9.5, 4096 -> 4096
+// 10.0 / 12.1, 6144 -> 3072 12.6 / 13.5, 3072 -> 9216 13.3 / 15.3; 3072 -> 12288
+// 17.7 / 17.1, 9216 -> 3072 17.5 / 16.4, 12288 -> 1024 17.5 / 11.8.
+bool dense_few_rows(int64_t R, int64_t C, int64_t L) {
+    return R <= kTileM || (R <= 2 * kTileM && L <= 6144 && C * L <= (int64_t(1) << 25));
+}
 
 int launch_dense_rows(const DenseProduct& a, cudaStream_t stream) {
     RowsParams p{};

@@ -112,6 +112,21 @@ def test_linear_every_row_count(m):
     check_linear(x, w, b, g, r, dy, "silu")
 
 
+@pytest.mark.parametrize("m", range(1, 18))
+@pytest.mark.parametrize("k,n", [(328, 264), (333, 57), (2048, 24)])
+def test_linear_few_rows(m, k, n):
+    # one and two tiles of rows, aligned and not, a gate per row; at 17 the other path
+    x, w, b, g, r, dy = make_linear(m, 1, k, n, torch.bfloat16, seed=m)
+    check_linear(x, w, b, g, r, dy, "gelu_tanh")
+    x, w, b, g, r, dy = make_linear(1, m, k, n + 1, torch.float16, seed=m, gate=False)
+    check_linear(x, w, b, g, r, dy, None)
+
+
+@pytest.mark.parametrize("k,n", [(6144, 136), (6145, 136), (6143, 40), (4096, 8192), (4096, 8193)])
+def test_linear_nine_rows_on_both_sides_of_the_rule(k, n):
+    check_linear(*make_linear(3, 3, k, n, torch.bfloat16), "silu")
+
+
 @pytest.mark.parametrize("k", [1, 2, 8, 15, 16, 24, 63, 64, 65, 127, 128, 136, 192, 1023])
 def test_linear_every_contraction_length(k):
     check_linear(*make_linear(1, 72, k, 80, torch.float16, seed=k), None)
