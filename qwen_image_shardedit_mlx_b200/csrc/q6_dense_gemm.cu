@@ -34,28 +34,35 @@ __global__ void __launch_bounds__(256) dense_reduce_kernel(const DenseParams p) 
     const int width = kVec ? p.C / 8 : p.C;
     const int64_t total = static_cast<int64_t>(p.R) * width;
     const int64_t plane = p.R * p.ld_partial;
+    const DenseEpilogue& e = p.epi;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        const int r = static_cast<int>(i / width), c = static_cast<int>(i % width) * (kVec ? 8 : 1);
+        const int r = static_cast<int>(total >> 32 ? i / width : static_cast<uint32_t>(i) / static_cast<uint32_t>(width));
+        const int c = static_cast<int>(i - int64_t(r) * width) * (kVec ? 8 : 1);
         const float* src = p.partial + r * p.ld_partial + c;
-        const int64_t gate_row = p.epi.gate ? r / p.gate_rows : 0;
+        const int gate_row = e.gate ? r / p.gate_rows : 0;
         if constexpr (kVec) {
+            Eight<T> bias{}, gate{}, res{};
+            if (e.bias) bias = load_ro<Eight<T>>(static_cast<const T*>(e.bias) + c);
+            if (e.gate) gate = load_ro<Eight<T>>(gate_at<T>(e, gate_row, c));
+            if (e.residual) res = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(e.residual) + r * e.ldr + c);
             float v[8] = {};
+#pragma unroll 4
             for (int s = 0; s < p.splits; ++s) {
                 const float4 a = *reinterpret_cast<const float4*>(src + s * plane);
                 const float4 b = *reinterpret_cast<const float4*>(src + s * plane + 4);
                 v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
                 v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
             }
-            Eight<T> bias{}, res{};
-            if (p.epi.bias) bias = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(p.epi.bias) + c);
-            if (p.epi.residual)
-                res = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(p.epi.residual) + r * p.epi.ldr + c);
-            finish8<T>(p.epi, p.d, r, p.C, c, gate_row, bias, res, v);
+            finish8<T>(e, p.d, r, p.C, c, bias, gate, res, v);
         } else {
-            float v[1] = {0.0f};
-            for (int s = 0; s < p.splits; ++s) v[0] += src[s * plane];
-            const float bias = p.epi.bias ? to_f(static_cast<const T*>(p.epi.bias)[c]) : 0.0f;
-            finish_column<T, 1, false>(p.epi, p.d, r, 1, p.C, c, p.gate_rows, bias, v);
+            T gate{}, res{};
+            const float bias = e.bias ? to_f(load_ro<T>(static_cast<const T*>(e.bias) + c)) : 0.0f;
+            if (e.gate) gate = load_ro<T>(gate_at<T>(e, gate_row, c));
+            if (e.residual) res = static_cast<const T*>(e.residual)[r * e.ldr + c];
+            float v = 0.0f;
+#pragma unroll 4
+            for (int s = 0; s < p.splits; ++s) v += src[s * plane];
+            finish1<T>(e, p.d, int64_t(r) * p.C + c, bias, gate, res, v);
         }
     }
 }

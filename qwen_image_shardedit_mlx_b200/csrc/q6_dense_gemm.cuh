@@ -22,7 +22,7 @@
 // The epilogue moves 32 x 32 blocks through shared memory (fp32, per warp), so
 // that each lane ends up with eight neighbouring outputs of a row: 16-byte
 // loads of bias, gate and residual and 16-byte stores.  Layouts that do not
-// allow that (odd widths, odd addresses) take one output per lane instead.
+// allow that (odd widths, odd addresses) take one column per lane instead.
 //
 // Every mbarrier wait is bounded (q6_ptx.cuh).
 #pragma once
@@ -158,27 +158,60 @@ struct alignas(16) Eight {
     T v[8];
 };
 
+// z of kCols neighbouring outputs, for the backward pass.
+template <int kCols>
+__device__ __forceinline__ void store_preact(const DenseEpilogue& e, int64_t at, const float* v) {
+    if (e.preact_f32) {
+        float* z = static_cast<float*>(e.preact) + at;
+        if constexpr (kCols == 8) {
+            reinterpret_cast<float4*>(z)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(z)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            *z = v[0];
+        }
+    } else {
+        __half* z = static_cast<__half*>(e.preact) + at;
+        if constexpr (kCols == 8) {
+            Eight<__half> g;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g.v[i] = preact_half(v[i]);
+            *reinterpret_cast<Eight<__half>*>(z) = g;
+        } else {
+            *z = preact_half(v[0]);
+        }
+    }
+}
+
+// A warp's block through shared memory, stage[row][column]: the 16-byte groups of
+// odd rows are swapped in pairs, so that the reads (two rows, every other group)
+// hit distinct banks.
+template <int kChunk>
+__device__ __forceinline__ void stage_block(float* stage, const uint32_t (&v)[kChunk]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) stage[j * 32 + (lane ^ ((j & 1) << 2))] = __uint_as_float(v[j]);
+    __syncwarp();
+}
+// Row j's eight columns from 8 (lane % 4) on.
+__device__ __forceinline__ void read_stage(const float* stage, int j, float* f) {
+    const int g = (threadIdx.x & 3) * 2, odd = j & 1;
+    const float4 a = *reinterpret_cast<const float4*>(stage + j * 32 + ((g ^ odd) << 2));
+    const float4 b = *reinterpret_cast<const float4*>(stage + j * 32 + (((g + 1) ^ odd) << 2));
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
 // Epilogue of eight neighbouring outputs of row r starting at column c.
 template <typename T>
-__device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t r, int64_t C, int c, int64_t gate_row,
-                                        const Eight<T>& bias, const Eight<T>& residual, float (&v)[8]) {
+__device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t r, int64_t C, int c,
+                                        const Eight<T>& bias, const Eight<T>& gate, const Eight<T>& residual,
+                                        float (&v)[8]) {
     if (e.bias) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], to_f(bias.v[i]));
     }
     const int64_t at = r * C + c;
-    if (e.preact) {
-        if (e.preact_f32) {
-            float4* z = reinterpret_cast<float4*>(static_cast<float*>(e.preact) + at);
-            z[0] = make_float4(v[0], v[1], v[2], v[3]);
-            z[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            Eight<__half> z;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z.v[i] = preact_half(v[i]);
-            *reinterpret_cast<Eight<__half>*>(static_cast<__half*>(e.preact) + at) = z;
-        }
-    }
+    if (e.preact) store_preact<8>(e, at, v);
     if (e.activation == Q6_ACT_GELU_TANH) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = act_f(v[i], Q6_ACT_GELU_TANH);
@@ -187,9 +220,8 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
         for (int i = 0; i < 8; ++i) v[i] = act_f(v[i], Q6_ACT_SILU);
     }
     if (e.gate) {
-        const Eight<T> g = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(e.gate) + gate_row * e.ldg + c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], to_f(g.v[i]));
+        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], to_f(gate.v[i]));
     }
     if (e.residual) {
 #pragma unroll
@@ -201,111 +233,268 @@ __device__ __forceinline__ void finish8(const DenseEpilogue& e, void* d, int64_t
     *reinterpret_cast<Eight<T>*>(static_cast<T*>(d) + at) = y;
 }
 
-// The same for kRows outputs of one column c (rows r .. r + n - 1 of them), any
-// layout; the rows' loads are issued together.  kPlain: a bias at most.
-template <typename T, int kRows, bool kPlain>
-__device__ __forceinline__ void finish_column(const DenseEpilogue& e, void* d, int r, int n, int64_t C, int c,
-                                              int gate_rows, float bias, float (&v)[kRows]) {
-    T* y = static_cast<T*>(d) + r * C + c;
-    if constexpr (kPlain) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i, y += C)
-            if (i < n) *y = from_f<T>(__fadd_rn(v[i], bias));
-    } else {
-        T res[kRows], gate[kRows];
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            if (i < n) {
-                if (e.residual) res[i] = static_cast<const T*>(e.residual)[(r + i) * e.ldr + c];
-                if (e.gate) gate[i] = static_cast<const T*>(e.gate)[(r + i) / gate_rows * e.ldg + c];
-            }
-        }
-        int64_t at = r * C + c;
-#pragma unroll
-        for (int i = 0; i < kRows; ++i, at += C, y += C) {
-            if (i < n) {
-                float t = __fadd_rn(v[i], bias);
-                if (e.preact) {
-                    if (e.preact_f32)
-                        static_cast<float*>(e.preact)[at] = t;
-                    else
-                        static_cast<__half*>(e.preact)[at] = preact_half(t);
-                }
-                t = act_f(t, e.activation);
-                if (e.gate) t = __fmul_rn(t, to_f(gate[i]));
-                if (e.residual) t = __fadd_rn(t, to_f(res[i]));
-                *y = from_f<T>(t);
-            }
-        }
-    }
+// The same for one output.
+template <typename T>
+__device__ __forceinline__ void finish1(const DenseEpilogue& e, void* d, int64_t at, float bias, T gate, T residual,
+                                        float v) {
+    v = __fadd_rn(v, bias);
+    if (e.preact) store_preact<1>(e, at, &v);
+    v = act_f(v, e.activation);
+    if (e.gate) v = __fmul_rn(v, to_f(gate));
+    if (e.residual) v = __fadd_rn(v, to_f(residual));
+    static_cast<T*>(d)[at] = from_f<T>(v);
 }
 
-// One warp's 32 columns (lanes of tensor memory) x kChunk rows.
-template <typename T, int kChunk>
-__device__ __forceinline__ void dense_epilogue_block(const DenseParams& p, const DenseItem& I, uint32_t taddr,
-                                                     float* stage, int r0, int c0, const Eight<T>& bias) {
-    const int lane = threadIdx.x & 31;
-    const DenseEpilogue& e = p.epi;
-    const int cv = c0 + (lane & 3) * 8;
-    Eight<T> res[kChunk / 8];
-    const bool to_partial = p.splits > 1;
-    if (p.vec && !to_partial && e.residual) {  // in flight while the accumulator is read
-#pragma unroll
-        for (int i = 0; i < kChunk / 8; ++i) {
-            const int r = r0 + i * 8 + (lane >> 2);
-            if (r < p.R && cv < p.C)
-                res[i] = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(e.residual) + r * e.ldr + cv);
-        }
-    }
-    uint32_t v[kChunk];
+template <typename T>
+__device__ __forceinline__ const T* gate_at(const DenseEpilogue& e, int64_t gate_row, int c) {
+    return static_cast<const T*>(e.gate) + gate_row * e.ldg + c;
+}
+
+// What one warp's block of the epilogue covers: 32 columns (lanes of tensor memory)
+// x kChunk rows.  By eight a lane has rows lane / 4, + 8, ... and eight columns from
+// c on, else every row and column c.
+struct DenseBlock {
+    int r0, rows, c;
+    bool inside, one_gate;  // c is a column of d; the rows share a gate vector
+    int gate_row;           // of the first row
+};
+
+template <int kChunk>
+__device__ __forceinline__ void load_accumulator(uint32_t taddr, uint32_t (&v)[kChunk]) {
+    __syncwarp();  // lanes outside the columns may have skipped loads
     if constexpr (kChunk == 32)
         tmem_ld_32x32b_x32(taddr, v);
     else
         tmem_ld_32x32b_x16(taddr, v);
     tmem_wait_ld();
-    // stage[row][column], the 16-byte groups of odd rows swapped in pairs so that
-    // the reads below (two rows, every other group) hit distinct banks
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) stage[j * 32 + (lane ^ ((j & 1) << 2))] = __uint_as_float(v[j]);
-    __syncwarp();
-    if (p.vec || to_partial) {
+}
+
+// A bias at most.  kAllRows: the block has all of its rows.
+template <typename T, int kChunk, bool kAllRows>
+__device__ __forceinline__ void dense_epilogue_plain(const DenseParams& p, const DenseBlock& B, uint32_t taddr,
+                                                     float* stage, const Eight<T>& bias8) {
+    const int lane = threadIdx.x & 31;
+    const DenseEpilogue& e = p.epi;
+    const float bias = !p.vec && e.bias && B.inside ? to_f(load_ro<T>(static_cast<const T*>(e.bias) + B.c)) : 0.0f;
+    uint32_t v[kChunk];
+    load_accumulator<kChunk>(taddr, v);
+    T* y = static_cast<T*>(p.d) + B.r0 * int64_t(p.C) + B.c;
+    if (p.vec) {
+        stage_block<kChunk>(stage, v);
 #pragma unroll
         for (int i = 0; i < kChunk / 8; ++i) {
-            const int j = i * 8 + (lane >> 2), g = (lane & 3) * 2, odd = j & 1;
-            const float4 a = *reinterpret_cast<const float4*>(stage + j * 32 + ((g ^ odd) << 2));
-            const float4 b = *reinterpret_cast<const float4*>(stage + j * 32 + (((g + 1) ^ odd) << 2));
-            float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            const int r = r0 + j;
-            if (r < p.R && cv < p.C) {
-                if (to_partial) {
-                    float4* dst = reinterpret_cast<float4*>(
-                        p.partial + (static_cast<int64_t>(I.split) * p.R + r) * p.ld_partial + cv);
-                    dst[0] = a;
-                    dst[1] = b;
+            const int j = i * 8 + (lane >> 2);
+            float f[8];
+            read_stage(stage, j, f);
+            Eight<T> out;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) out.v[k] = from_f<T>(e.bias ? __fadd_rn(f[k], to_f(bias8.v[k])) : f[k]);
+            if ((kAllRows || j < B.rows) && B.inside) *reinterpret_cast<Eight<T>*>(y + j * int64_t(p.C)) = out;
+        }
+        __syncwarp();
+    } else if (B.inside) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i, y += p.C)
+            if (kAllRows || i < B.rows) *y = from_f<T>(e.bias ? __fadd_rn(__uint_as_float(v[i]), bias) : __uint_as_float(v[i]));
+    }
+}
+
+// A block with all of its rows, one gate vector at most: straight passes over
+// sixteen of the lane's values, without a condition per row, so that their
+// latencies overlap (an SM has eight epilogue warps).  What the passes read is
+// loaded one turn ahead; the residual so before the rows of y, which may lie in it,
+// are written.  In turns of sixteen because a short sum runs the epilogue once per
+// CTA, and its time is then that of fetching its instructions: with all 32 values
+// in one turn 580 x 240 -> 2696 (GELU, gate, residual) took 14.4 us, 11.3 so;
+// 8192 x 1001 -> 777 (gate, residual), which the latencies bound, 51 and 46, and 118
+// with loops over the rows.
+template <typename T, int kChunk, bool kEight>
+__device__ __forceinline__ void dense_epilogue_full(const DenseParams& p, const DenseBlock& B, uint32_t taddr, float* stage,
+                                                    const Eight<T>& bias8) {
+    constexpr int kPart = 16, kRows = kEight ? kPart / 8 : kPart, kCols = kEight ? 8 : 1;
+    const int lane = threadIdx.x & 31;
+    const DenseEpilogue& e = p.epi;
+    const int first = B.r0 + (kEight ? lane >> 2 : 0), step = kEight ? 8 : 1;
+    const T* from = static_cast<const T*>(e.residual) + first * e.ldr + B.c;
+    Eight<T> gate{}, next[2];
+    float bias = 0.0f;
+    auto load_residual = [&] {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i, from += step * e.ldr) {
+            if constexpr (kEight)
+                next[i] = *reinterpret_cast<const Eight<T>*>(from);
+            else
+                next[i / 8].v[i % 8] = *from;
+        }
+    };
+    if (B.inside) {
+        if (e.residual) load_residual();
+        if (e.gate) {
+            if constexpr (kEight)
+                gate = load_ro<Eight<T>>(gate_at<T>(e, B.gate_row, B.c));
+            else
+                gate.v[0] = load_ro<T>(gate_at<T>(e, B.gate_row, B.c));
+        }
+        if (!kEight && e.bias) bias = to_f(load_ro<T>(static_cast<const T*>(e.bias) + B.c));
+    }
+    uint32_t v[kChunk];
+    load_accumulator<kChunk>(taddr, v);
+    const int64_t row = step * int64_t(p.C);
+    int64_t at = first * int64_t(p.C) + B.c;
+    stage_block<kChunk>(stage, v);
+    if (B.inside) {
+#pragma unroll 1
+        for (int h = 0; h < kChunk / kPart; ++h) {
+            const Eight<T> res[2] = {next[0], next[1]};
+            if (e.residual && h + 1 < kChunk / kPart) load_residual();
+            float f[kPart];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                if constexpr (kEight)
+                    read_stage(stage, h * kPart + i * 8 + (lane >> 2), f + 8 * i);
+                else
+                    f[i] = stage[(h * kPart + i) * 32 + (lane ^ ((i & 1) << 2))];
+            }
+            if (e.bias) {
+#pragma unroll
+                for (int i = 0; i < kPart; ++i) f[i] = __fadd_rn(f[i], kEight ? to_f(bias8.v[i % 8]) : bias);
+            }
+            if (e.preact) {
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) store_preact<kCols>(e, at + i * row, f + kCols * i);
+            }
+            if (e.activation == Q6_ACT_GELU_TANH) {
+#pragma unroll
+                for (int i = 0; i < kPart; ++i) f[i] = act_f(f[i], Q6_ACT_GELU_TANH);
+            } else if (e.activation == Q6_ACT_SILU) {
+#pragma unroll
+                for (int i = 0; i < kPart; ++i) f[i] = act_f(f[i], Q6_ACT_SILU);
+            }
+            if (e.gate) {
+#pragma unroll
+                for (int i = 0; i < kPart; ++i) f[i] = __fmul_rn(f[i], to_f(gate.v[kEight ? i % 8 : 0]));
+            }
+            if (e.residual) {
+#pragma unroll
+                for (int i = 0; i < kPart; ++i) f[i] = __fadd_rn(f[i], to_f(res[i / 8].v[i % 8]));
+            }
+            T* y = static_cast<T*>(p.d) + at;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i, y += row) {
+                if constexpr (kEight) {
+                    Eight<T> out;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) out.v[k] = from_f<T>(f[8 * i + k]);
+                    *reinterpret_cast<Eight<T>*>(y) = out;
                 } else {
-                    finish8<T>(e, p.d, r, p.C, cv, e.gate ? r / p.gate_rows : 0, bias, res[i], f);
+                    *y = from_f<T>(f[i]);
                 }
             }
+            at += kRows * row;
         }
-    } else {
-        const int c = c0 + lane;
-        if (c < p.C) {
-            const float b = e.bias ? to_f(static_cast<const T*>(e.bias)[c]) : 0.0f;
-            const bool plain = !e.preact && e.activation == Q6_ACT_NONE && !e.gate && !e.residual;
+    }
+    __syncwarp();
+}
+
+// Any block of outputs, by eight or one.
+template <typename T, int kChunk>
+__device__ __forceinline__ void dense_epilogue_ragged(const DenseParams& p, const DenseBlock& B, uint32_t taddr,
+                                                      float* stage, const Eight<T>& bias8) {
+    const int lane = threadIdx.x & 31;
+    const DenseEpilogue& e = p.epi;
+    uint32_t v[kChunk];
+    load_accumulator<kChunk>(taddr, v);
+    stage_block<kChunk>(stage, v);
+    if (B.inside) {
+        if (p.vec) {
 #pragma unroll 1
-            for (int j = 0; j < kChunk && r0 + j < p.R; j += 8) {
+            for (int j = lane >> 2; j < B.rows; j += 8) {
+                const int r = B.r0 + j;
+                Eight<T> gate{}, res{};
+                if (e.gate) gate = load_ro<Eight<T>>(gate_at<T>(e, r / p.gate_rows, B.c));
+                if (e.residual)
+                    res = *reinterpret_cast<const Eight<T>*>(static_cast<const T*>(e.residual) + r * e.ldr + B.c);
                 float f[8];
+                read_stage(stage, j, f);
+                finish8<T>(e, p.d, r, p.C, B.c, bias8, gate, res, f);
+            }
+        } else {
+            const float bias = e.bias ? to_f(load_ro<T>(static_cast<const T*>(e.bias) + B.c)) : 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < B.rows; j += 4) {
+                T gate[4], res[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = stage[(j + i) * 32 + (lane ^ ((i & 1) << 2))];
-                const int n = min(8, p.R - r0 - j);
-                if (plain && n == 8)
-                    finish_column<T, 8, true>(e, p.d, r0 + j, 8, p.C, c, p.gate_rows, b, f);
-                else
-                    finish_column<T, 8, false>(e, p.d, r0 + j, n, p.C, c, p.gate_rows, b, f);
+                for (int i = 0; i < 4; ++i) {
+                    const int r = B.r0 + j + i;
+                    if (j + i < B.rows) {
+                        if (e.gate) gate[i] = load_ro<T>(gate_at<T>(e, r / p.gate_rows, B.c));
+                        if (e.residual) res[i] = static_cast<const T*>(e.residual)[r * e.ldr + B.c];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (j + i < B.rows)
+                        finish1<T>(e, p.d, (B.r0 + j + i) * int64_t(p.C) + B.c, bias, gate[i], res[i],
+                                   stage[(j + i) * 32 + (lane ^ ((i & 1) << 2))]);
             }
         }
     }
     __syncwarp();
+}
+
+// kPlain: a product with no epilogue (the gradients').
+template <typename T, int kChunk, bool kPlain>
+__device__ __forceinline__ void dense_epilogue_block(const DenseParams& p, const DenseItem& I, uint32_t taddr,
+                                                     float* stage, int r0, int c0, const Eight<T>& bias) {
+    const int lane = threadIdx.x & 31;
+    DenseBlock B;
+    B.r0 = r0;
+    B.rows = min(kChunk, p.R - r0);
+    if (p.splits > 1) {
+        float* to = p.partial + (static_cast<int64_t>(I.split) * p.R + r0) * p.ld_partial;
+        const int c = c0 + (lane & 3) * 8;
+        uint32_t v[kChunk];
+        load_accumulator<kChunk>(taddr, v);
+        stage_block<kChunk>(stage, v);
+#pragma unroll
+        for (int i = 0; i < kChunk / 8; ++i) {  // by eight: a partial row is padded to that
+            const int j = i * 8 + (lane >> 2);
+            if (j < B.rows && c < p.C) {
+                float f[8];
+                read_stage(stage, j, f);
+                float4* dst = reinterpret_cast<float4*>(to + j * p.ld_partial + c);
+                dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+                dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+            }
+        }
+        __syncwarp();
+        return;
+    }
+    B.c = c0 + (p.vec ? (lane & 3) * 8 : lane);
+    B.inside = B.c < p.C;
+    const bool all_rows = B.rows == kChunk;
+    if constexpr (kPlain) {
+        if (all_rows)
+            dense_epilogue_plain<T, kChunk, true>(p, B, taddr, stage, bias);
+        else
+            dense_epilogue_plain<T, kChunk, false>(p, B, taddr, stage, bias);
+    } else {
+        const DenseEpilogue& e = p.epi;
+        B.gate_row = 0;
+        B.one_gate = true;
+        if (e.gate) {
+            B.gate_row = r0 / p.gate_rows;
+            B.one_gate = (r0 + B.rows - 1) / p.gate_rows == B.gate_row;
+        }
+        if (!all_rows || !B.one_gate)
+            dense_epilogue_ragged<T, kChunk>(p, B, taddr, stage, bias);
+        else if (!e.preact && e.activation == Q6_ACT_NONE && !e.gate && !e.residual)
+            dense_epilogue_plain<T, kChunk, true>(p, B, taddr, stage, bias);
+        else if (p.vec)
+            dense_epilogue_full<T, kChunk, true>(p, B, taddr, stage, bias);
+        else
+            dense_epilogue_full<T, kChunk, false>(p, B, taddr, stage, bias);
+    }
 }
 
 template <int CT, bool kPair, bool kPT, bool kQT>
@@ -515,11 +704,12 @@ __global__ void __launch_bounds__(kDenseThreads, 1)
                 const int r0 = I.r * CT + ch * C::kChunk;
                 if (r0 >= p.R) break;  // the same for the whole warp
                 if (p.half)
-                    dense_epilogue_block<__half, C::kChunk>(p, I, taddr + ch * C::kChunk, stage, r0, c0,
-                                                            *reinterpret_cast<const Eight<__half>*>(&bias));
+                    dense_epilogue_block<__half, C::kChunk, kPT>(p, I, taddr + ch * C::kChunk, stage, r0, c0,
+                                                                 *reinterpret_cast<const Eight<__half>*>(&bias));
                 else
-                    dense_epilogue_block<__nv_bfloat16, C::kChunk>(p, I, taddr + ch * C::kChunk, stage, r0, c0,
-                                                                   *reinterpret_cast<const Eight<__nv_bfloat16>*>(&bias));
+                    dense_epilogue_block<__nv_bfloat16, C::kChunk, kPT>(
+                        p, I, taddr + ch * C::kChunk, stage, r0, c0,
+                        *reinterpret_cast<const Eight<__nv_bfloat16>*>(&bias));
             }
             tc_fence_before();
             __syncwarp();

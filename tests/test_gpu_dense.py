@@ -10,7 +10,7 @@ import torch
 
 import bounds
 from bounds import B
-from qwen_image_shardedit_mlx_b200 import dense, ops
+from qwen_image_shardedit_mlx_b200 import _lib, dense, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -323,6 +323,25 @@ def test_linear_capture_with_gradients_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, dense.dense_linear(x, w.detach(), b))
+
+
+@pytest.mark.parametrize("m,k,n", [(5, 136, 72), (13, 130, 71), (300, 264, 520), (300, 263, 521), (96, 4096, 136), (96, 4096, 131)])
+def test_output_in_place_of_the_residual(m, k, n):
+    # the C entry may write y over the residual: few rows, whole and ragged blocks, split sums, odd widths
+    lib = _lib.lib()
+    x, w, b, _, _, _ = make_linear(1, m, k, n, torch.bfloat16, gate=False)
+    r = rand((m, n), torch.bfloat16, 9)
+    g = rand((n,), torch.bfloat16, 10)
+    want = dense.dense_linear(x[0], w, b, activation="silu", gate=g, residual=r)
+    pack = (_lib.Q6_PACK_X | _lib.Q6_PACK_W) if k % 8 else 0
+    nbytes = lib.q6_dense_linear_workspace_bytes(m, n, k, pack)
+    ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device="cuda")
+    status = lib.q6_dense_linear(x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), g.data_ptr(), n, m, r.data_ptr(), n,
+                                 r.data_ptr(), None, _lib.Q6_DTYPE_F16, m, n, k, _lib.Q6_DTYPE_BF16, _lib.Q6_ACT_SILU,
+                                 ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+    assert status == 0
+    torch.cuda.synchronize()
+    assert torch.equal(r, want)
 
 
 def test_captured_backward_of_an_eager_call_is_refused():
