@@ -356,16 +356,24 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
     const int tiles = (rows + TR - 1) / TR;
     const T* x = static_cast<const T*>(p.x) + r_begin * p.ldx;
     const T* dy = static_cast<const T*>(p.dy) + r_begin * p.ldy;
-    // tile i into stage s, by one warp: a lane per row copy
+    // tile i (its rows of x, then those of dy) into stage s, by one warp: rows that
+    // lie together in one copy (a copy per row: 165888 x 128 123 us, 65 so), else a
+    // lane per row copy
+    const bool whole_x = p.ldx == D, whole_dy = p.ldy == D;
     auto fill = [&](int i, int s) {
         const int n = min(TR, rows - i * TR);
-        const uint32_t bar = smem_u32(full + s), to = smem_u32(smem) + s * tile_bytes;
-        if (lane == 0) mbar_arrive_expect_tx(bar, n * 2 * row_bytes);
-        __syncwarp();
-        for (int k = lane; k < 2 * n; k += 32) {
-            const int64_t r = i * TR + (k >> 1);
-            bulk_load(to + k * row_bytes, (k & 1) ? static_cast<const void*>(dy + r * p.ldy) : x + r * p.ldx, row_bytes, bar);
+        const int64_t r0 = int64_t(i) * TR;
+        const uint32_t bar = smem_u32(full + s), to_x = smem_u32(smem) + s * tile_bytes, to_dy = to_x + TR * row_bytes;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bar, n * 2 * row_bytes);
+            if (whole_x) bulk_load(to_x, x + r0 * p.ldx, n * row_bytes, bar);
+            if (whole_dy) bulk_load(to_dy, dy + r0 * p.ldy, n * row_bytes, bar);
         }
+        __syncwarp();
+        if (!whole_x)
+            for (int k = lane; k < n; k += 32) bulk_load(to_x + k * row_bytes, x + (r0 + k) * p.ldx, row_bytes, bar);
+        if (!whole_dy)
+            for (int k = lane; k < n; k += 32) bulk_load(to_dy + k * row_bytes, dy + (r0 + k) * p.ldy, row_bytes, bar);
     };
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) mbar_init(smem_u32(full + s), 1);
@@ -428,8 +436,8 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
         for (int k = 0; k < AR; ++k) {
             const int r = a_row + k * kStep;
             if (r < n) {
-                const T* xr = reinterpret_cast<const T*>(tile + (2 * r) * row_bytes);
-                const T* yr = reinterpret_cast<const T*>(tile + (2 * r + 1) * row_bytes);
+                const T* xr = reinterpret_cast<const T*>(tile + r * row_bytes);
+                const T* yr = reinterpret_cast<const T*>(tile + (TR + r) * row_bytes);
                 const float2 neg_mean = both(-mean[k]);
                 float2 sa = both(0.0f), st = both(0.0f);
 #pragma unroll
@@ -494,8 +502,8 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
                     row.w = scale * row.y * row.y * m.y;
                 }
                 const float2 neg_mean = both(row.x), rstd = both(row.y), kc = both(row.z), kt = both(row.w);
-                const T* xr = reinterpret_cast<const T*>(tile + (2 * r) * row_bytes);
-                const T* yr = reinterpret_cast<const T*>(tile + (2 * r + 1) * row_bytes);
+                const T* xr = reinterpret_cast<const T*>(tile + r * row_bytes);
+                const T* yr = reinterpret_cast<const T*>(tile + (TR + r) * row_bytes);
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     if (at.some(j)) {
