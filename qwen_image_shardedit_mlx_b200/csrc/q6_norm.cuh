@@ -92,9 +92,11 @@ __device__ __forceinline__ void warp_sum2(float2& a, float2& b) {
     b.y = __shfl_sync(0xffffffffu, s, 3);
 }
 
-__device__ __forceinline__ float warp_sum1(float v) {
+// Sum over each run of L lanes.
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
@@ -161,27 +163,32 @@ struct Columns {
     }
 };
 
-// Forward: W warps per row (one row per CTA; four with W = 1), N groups per
-// thread.  N is at most four: a row's code runs once per row, and with twelve
+// Forward: W warps per row (one row per CTA), or L lanes (128 / L rows per CTA; a
+// row of 128 in a warp of its own left half its lanes idle: 165888 rows of bf16
+// 37.6 us, 20.4 so), N groups per thread.  N is at most four: a row's code runs once per row, and with twelve
 // groups per lane (a warp per row of 3072) its unrolled length ran out of the
 // instruction cache: 31 us for 6912 rows of bf16 against 21 us with four.  The
 // grid is one wave of CTAs that walk the rows, the next row's loads in flight
 // while a row is summed: 15.7 us (5.4 TB/s).
-template <typename T, typename V, Layout kLay, int W, int N>
+template <typename T, typename V, Layout kLay, int W, int N, int L>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormParams p) {
-    constexpr int G = 16 / sizeof(T), kRows = W == 1 ? 4 : 1;
+    constexpr int G = 16 / sizeof(T), kRows = W == 1 ? 128 / L : 1;
+    static_assert(L == 32 || W == 1, "lanes of one warp");
     __shared__ float parts[2][W];
     pdl_launch_dependents();
     // rows first, first + step, ... of a vector's rows, or of all where the vectors are not the grid's second axis
     const int64_t limit = p.vecs ? p.rows_per_vec : p.M, step = gridDim.x * int64_t(kRows);
-    int64_t local = W == 1 ? blockIdx.x * int64_t(kRows) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
-    if (local >= limit) return;  // a whole warp of a CTA of single-warp rows
+    int64_t local = W == 1 ? blockIdx.x * int64_t(kRows) + threadIdx.x / L : int64_t(blockIdx.x);
+    int64_t warp_row = W == 1 ? blockIdx.x * int64_t(kRows) + threadIdx.x / 32 * (32 / L) : int64_t(blockIdx.x);
+    if (warp_row >= limit) return;  // a whole warp
+    // lanes past the last row follow their warp on that row, and store nothing
+    auto row_of = [&](int64_t r) { return L < 32 ? min(r, limit - 1) : r; };
     const int64_t row0 = p.vecs ? blockIdx.y * p.rows_per_vec : 0;
     pdl_wait();
-    const Columns<T, kLay, 32 * W> at{W == 1 ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
-                                      static_cast<int>(p.D)};
+    const Columns<T, kLay, L * W> at{W == 1 ? static_cast<int>(threadIdx.x % L) : static_cast<int>(threadIdx.x),
+                                     static_cast<int>(p.D)};
     auto row_sum = [&](float v, int flip) {
-        v = warp_sum1(v);
+        v = lanes_sum<L>(v);
         if constexpr (W > 1) {
             if ((at.t & 31) == 0) parts[flip][at.t >> 5] = v;
             __syncthreads();
@@ -191,17 +198,20 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormP
         }
         return v;
     };
-    const T* x = static_cast<const T*>(p.x) + (row0 + local) * p.ldx;
+    const T* x = static_cast<const T*>(p.x) + (row0 + row_of(local)) * p.ldx;
     Group<T, G> in[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) in[j] = at.load(x, j);
     const float inv = 1.0f / static_cast<float>(at.D);
-    for (;; local += step) {
-        const int64_t row = row0 + local;
-        const bool more = local + step < limit;
+    for (;; local += step, warp_row += step) {
+        const int64_t row = row0 + row_of(local);
+        const bool more = warp_row + step < limit, ours = L == 32 || local < limit;
         Group<T, G> next[N];
         if (more) {
-            x += step * p.ldx;
+            if constexpr (L == 32)
+                x += step * p.ldx;
+            else
+                x = static_cast<const T*>(p.x) + (row0 + row_of(local + step)) * p.ldx;
 #pragma unroll
             for (int j = 0; j < N; ++j) next[j] = at.load(x, j);
         }
@@ -239,14 +249,14 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormP
             }
         }
         const float rstd = rsqrtf(row_sum(q.x + q.y, 1) * inv + p.eps);
-        if (p.mean && at.t == 0) {
+        if (p.mean && at.t == 0 && ours) {
             p.mean[row] = mean;
             p.rstd[row] = rstd;
         }
         T* y = static_cast<T*>(p.y) + row * p.D;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            if (at.some(j)) {
+            if (ours && at.some(j)) {
                 float2 fw[G / 2], fb[G / 2];
                 at.factor(w, j, p.one, fw);
 #pragma unroll
@@ -628,11 +638,13 @@ __global__ void __launch_bounds__(32 * CW * (CW < 16 ? 16 / CW : 1), 1)
 // ------------------------------------------------------------------- host side
 
 // W warps x N groups per thread cover a row (m: rows per thread and tile of the
-// backward); the first entry that covers the row's groups of G elements.
+// backward; lanes: of the warp, for one row); the first entry that covers the
+// row's groups of G elements.
 struct NormShape {
-    int w, n, m;
+    int w, n, m = 1, lanes = 32;
 };
-constexpr NormShape kNormForward[] = {{1, 1}, {1, 2}, {1, 4}, {2, 4}, {3, 4}, {4, 4}, {6, 4}, {8, 4}, {12, 4}, {16, 4}, {32, 4}};
+constexpr NormShape kNormForward[] = {{1, 1, 1, 4}, {1, 1, 1, 8}, {1, 1, 1, 16}, {1, 1}, {1, 2},  {1, 4},  {2, 4},
+                                      {3, 4},       {4, 4},       {6, 4},        {8, 4}, {12, 4}, {16, 4}, {32, 4}};
 constexpr NormShape kNormGrad[] = {{1, 1, 4}, {1, 2, 2}, {2, 2, 2},  {3, 2, 3},  {4, 2, 2}, {6, 2, 2},
                                    {8, 2, 2}, {12, 2, 2}, {16, 2, 2}, {12, 4, 1}, {16, 4, 1}};
 constexpr NormShape kNormGradStrided[] = {{1, 1, 1}, {1, 2, 1}, {2, 2, 1}, {4, 2, 1}, {8, 2, 1}, {16, 2, 1}, {16, 4, 1}};
@@ -642,7 +654,7 @@ template <size_t K>
 int norm_shape(const NormShape (&list)[K], int64_t D, int dtype) {
     const int64_t g = dtype == Q6_DTYPE_F32 ? 4 : 8, groups = (D + g - 1) / g;
     for (size_t i = 0; i < K; ++i)
-        if (groups <= int64_t(32) * list[i].w * list[i].n) return static_cast<int>(i);
+        if (groups <= int64_t(list[i].lanes) * list[i].w * list[i].n) return static_cast<int>(i);
     return -1;  // the plain kernels
 }
 
@@ -657,9 +669,9 @@ int norm_forward_typed(const NormParams& p, bool vec, int shape, cudaStream_t st
 template <typename T, typename V>
 int norm_grad_typed(const NormParams& p, bool vec, int shape, V* dweight, V* dbias, cudaStream_t stream);
 
-template <typename T, typename V, norm_detail::Layout kLay, int W, int N>
+template <typename T, typename V, norm_detail::Layout kLay, int W, int N, int L>
 int launch_norm_forward(const NormParams& p, cudaStream_t stream) {
-    auto* kernel = norm_detail::norm_kernel<T, V, kLay, W, N>;
+    auto* kernel = norm_detail::norm_kernel<T, V, kLay, W, N, L>;
     constexpr int threads = W == 1 ? 128 : 32 * W;
     // CTAs per SM, looked up once per device
     static std::atomic<int> resident[kMaxDevices];
@@ -672,7 +684,7 @@ int launch_norm_forward(const NormParams& p, cudaStream_t stream) {
             return Q6_ERR_CUDA;
         resident[dev].store(per_sm, std::memory_order_relaxed);
     }
-    const int64_t rows = p.vecs ? p.rows_per_vec : p.M, vecs = p.vecs ? p.vecs : 1, per = W == 1 ? 4 : 1;
+    const int64_t rows = p.vecs ? p.rows_per_vec : p.M, vecs = p.vecs ? p.vecs : 1, per = W == 1 ? 128 / L : 1;
     const int64_t wave = std::max<int64_t>(1, int64_t(device_sm_count()) * per_sm / vecs);
     return launch_pdl(kernel, dim3(static_cast<unsigned>(std::min((rows + per - 1) / per, wave)), p.vecs ? p.vecs : 1u),
                       dim3(threads), 0, stream, p) == cudaSuccess
@@ -726,11 +738,12 @@ int launch_norm_grad_strided(const NormParams& p, V* dweight, V* dbias, cudaStre
                : Q6_ERR_CUDA;
 }
 
-template <typename T, typename V, int W, int N>
+template <typename T, typename V, int W, int N, int L>
 int norm_forward_layout(const NormParams& p, bool vec, cudaStream_t stream) {
     using namespace norm_detail;
-    if (vec && p.D == 32 * W * N * int64_t(16 / sizeof(T))) return launch_norm_forward<T, V, kFull, W, N>(p, stream);
-    return vec ? launch_norm_forward<T, V, kVec, W, N>(p, stream) : launch_norm_forward<T, V, kStrided, W, N>(p, stream);
+    if (vec && p.D == L * W * N * int64_t(16 / sizeof(T))) return launch_norm_forward<T, V, kFull, W, N, L>(p, stream);
+    return vec ? launch_norm_forward<T, V, kVec, W, N, L>(p, stream)
+               : launch_norm_forward<T, V, kStrided, W, N, L>(p, stream);
 }
 
 template <typename T, typename V, int W, int N, int M>
@@ -744,7 +757,7 @@ template <typename T, typename V, size_t... I>
 int norm_forward_list(const NormParams& p, bool vec, int shape, cudaStream_t stream, std::index_sequence<I...>) {
     int st = Q6_ERR_UNSUPPORTED;
     ((shape == int(I) &&
-      (st = norm_forward_layout<T, V, kNormForward[I].w, kNormForward[I].n>(p, vec, stream), true)) ||
+      (st = norm_forward_layout<T, V, kNormForward[I].w, kNormForward[I].n, kNormForward[I].lanes>(p, vec, stream), true)) ||
      ...);
     return st;
 }

@@ -415,7 +415,7 @@ def make_norm(samples, rows, d, dtype, vec_dtype, *, per_sample, seed=0):
 
 NORM = [(1, 1, 1), (1, 1, 8), (1, 5, 3), (2, 7, 33), (1, 9, 64), (3, 50, 100), (1, 333, 129), (2, 40, 256), (1, 17, 1001),
         (2, 21, 1024), (1, 64, 1152), (1, 70, 2048), (2, 33, 3072), (1, 12, 4096), (1, 5, 8192), (1, 3, 12288),
-        (1, 2, 20001), (1, 2, 16384), (700, 1, 40), (1, 3000, 72)]
+        (1, 2, 20001), (1, 2, 16384), (700, 1, 40), (1, 3000, 72), (5, 301, 128), (3, 1003, 16), (2, 259, 31), (1, 20003, 64)]
 
 
 @pytest.mark.parametrize("shape", NORM, ids=lambda s: "x".join(map(str, s)))
