@@ -165,11 +165,11 @@ struct Columns {
 
 // Forward: W warps per row (one row per CTA), or L lanes (128 / L rows per CTA; a
 // row of 128 in a warp of its own left half its lanes idle: 165888 rows of bf16
-// 37.6 us, 20.4 so), N groups per thread.  N is at most four: a row's code runs once per row, and with twelve
-// groups per lane (a warp per row of 3072) its unrolled length ran out of the
-// instruction cache: 31 us for 6912 rows of bf16 against 21 us with four.  The
-// grid is one wave of CTAs that walk the rows, the next row's loads in flight
-// while a row is summed: 15.7 us (5.4 TB/s).
+// 37.6 us, 20.4 so), N groups per thread.  N is at most four: a row's code runs
+// once per row, and with twelve groups per lane (a warp per row of 3072) its
+// unrolled length ran out of the instruction cache: 31 us for 6912 rows of bf16
+// against 21 us with four.  The grid is one wave of CTAs that walk the rows, the
+// next row's loads in flight while a row is summed: 15.5 us (5.5 TB/s).
 template <typename T, typename V, Layout kLay, int W, int N, int L>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormParams p) {
     constexpr int G = 16 / sizeof(T), kRows = W == 1 ? 128 / L : 1;
