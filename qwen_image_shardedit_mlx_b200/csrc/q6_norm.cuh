@@ -326,7 +326,7 @@ __device__ __forceinline__ void finish_columns(const NormParams& p, const C& at,
 
 // Backward.  A CTA takes one strip of rows (all of one vector) in tiles of
 // TR = RL * M rows, in two phases with one barrier between them:
-//   A  every row of the tile is summed by CW / M warps (sum a, sum a (x - mean));
+//   A  every row of the tile is summed by CW / M warps (sum a, sum a xh);
 //   B  every thread keeps N groups of columns (CW warps cover the row, RL row
 //      lanes side by side) for M rows of the tile: dx, and the column sums of
 //      dy xh and dy in registers.
@@ -335,8 +335,12 @@ __device__ __forceinline__ void finish_columns(const NormParams& p, const C& at,
 // after its last read of the stage.  With x and dy held in registers and a
 // barrier per row instead, 6912 rows of 3072 took 46 us: a row's chain of
 // shuffles, barrier and sums left the SM idle.
-//   In B: with u = dy rstd and t = x - mean,
-//   dx = u w + t k + c,  k = -rstd^2 mean_D(a xh),  c = -rstd mean_D(a);  dweight += u t.
+//   In B: dx = rstd (dy w + xh k + c),  k = -mean_D(a xh),  c = -mean_D(a);  dweight += dy xh.
+// Both phases form xh = (x - mean) rstd before anything is multiplied with it, and rstd
+// enters dx last: every intermediate value then has the scale of an input or output.  (With
+// sums of a (x - mean) and a coefficient rstd^2 mean_D(a xh) a multiply per pair of values
+// is saved, but rstd^3 leaves fp32 on the way: rows of a standard deviation from 1e13 on
+// lost the third term, rows of 1e-14 with eps = 0 gave infinities.)
 // Row lanes: about 384 threads.  Fewer threads mean smaller tiles, so more of
 // them in flight: with 576, two stages of 72 KB, a tile's copy had half a tile's
 // time to land (65536 x 1024 fp16 110 us, 80 so; 256 threads 96).
@@ -448,8 +452,8 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
             if (r < n) {
                 const T* xr = reinterpret_cast<const T*>(tile + r * row_bytes);
                 const T* yr = reinterpret_cast<const T*>(tile + (TR + r) * row_bytes);
-                const float2 neg_mean = both(-mean[k]);
-                float2 sa = both(0.0f), st = both(0.0f);
+                const float2 neg_mean = both(-mean[k]), scale = both(rstd[k]);
+                float2 sa = both(0.0f), sh = both(0.0f);
 #pragma unroll
                 for (int j = 0; j < N * CW / AP; ++j) {
                     const int g = (j * AP + a_part) * 32 + lane;
@@ -463,17 +467,16 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
                             const float2 a0 = mul2(fy[e], make_float2(f.x, f.y)),
                                          a1 = mul2(fy[e + 1], make_float2(f.z, f.w));
                             sa = add2(sa, a0);
-                            st = fma2(a0, add2(fx[e], neg_mean), st);
+                            sh = fma2(a0, mul2(add2(fx[e], neg_mean), scale), sh);
                             sa = add2(sa, a1);
-                            st = fma2(a1, add2(fx[e + 1], neg_mean), st);
+                            sh = fma2(a1, mul2(add2(fx[e + 1], neg_mean), scale), sh);
                         }
                     }
                 }
-                const float2 m = warp_sum2(make_float2(sa.x + sa.y, st.x + st.y));
+                const float2 m = warp_sum2(make_float2(sa.x + sa.y, sh.x + sh.y));
                 if (lane == 0) {
                     if constexpr (AP == 1) {
-                        const float scale = -rstd[k] * inv;
-                        stats[flip][r] = make_float4(-mean[k], rstd[k], scale * m.x, scale * rstd[k] * rstd[k] * m.y);
+                        stats[flip][r] = make_float4(-mean[k], rstd[k], -m.x * inv, -m.y * inv);
                     } else {
                         parts[flip][r][a_part] = m;
                         if (a_part == 0) stats[flip][r] = make_float4(-mean[k], rstd[k], 0.0f, 0.0f);
@@ -507,11 +510,10 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
 #pragma unroll
                         for (int k = 1; k < AP; ++k) m = add2(m, parts[flip][r][k]);
                     }
-                    const float scale = -row.y * inv;
-                    row.z = scale * m.x;
-                    row.w = scale * row.y * row.y * m.y;
+                    row.z = -m.x * inv;
+                    row.w = -m.y * inv;
                 }
-                const float2 neg_mean = both(row.x), rstd = both(row.y), kc = both(row.z), kt = both(row.w);
+                const float2 neg_mean = both(row.x), rstd = both(row.y), kc = both(row.z), kh = both(row.w);
                 const T* xr = reinterpret_cast<const T*>(tile + r * row_bytes);
                 const T* yr = reinterpret_cast<const T*>(tile + (TR + r) * row_bytes);
 #pragma unroll
@@ -522,10 +524,10 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
                         unpack(load_shared<T, G>(yr + at.column(j, 0)), fy);
 #pragma unroll
                         for (int e = 0; e < P; ++e) {
-                            const float2 u = mul2(fy[e], rstd), t = add2(fx[e], neg_mean);
+                            const float2 h = mul2(add2(fx[e], neg_mean), rstd);
                             db[j][e] = add2(db[j][e], fy[e]);
-                            dw[j][e] = fma2(u, t, dw[j][e]);
-                            fx[e] = fma2(u, fw[j][e], fma2(t, kt, kc));
+                            dw[j][e] = fma2(fy[e], h, dw[j][e]);
+                            fx[e] = mul2(fma2(fy[e], fw[j][e], fma2(h, kh, kc)), rstd);
                         }
                         if (dx) at.store(dx + (static_cast<int64_t>(i) * TR + q * RL) * p.D, j, pack<T, G>(fx));
                     }
@@ -605,7 +607,7 @@ __global__ void __launch_bounds__(32 * CW * (CW < 16 ? 16 / CW : 1), 1)
 #pragma unroll
             for (int k = 1; k < CW; ++k) m = add2(m, parts[flip][group][k]);
         }
-        const float2 ka = both(-rstd * m.x * inv), kh = both(-rstd * m.y * inv);
+        const float2 ka = both(-m.x * inv), kh = both(-m.y * inv);
         // unpack the row again: in fp32 it would not fit the registers
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -622,8 +624,8 @@ __global__ void __launch_bounds__(32 * CW * (CW < 16 ? 16 / CW : 1), 1)
                 unpack(gy[j], fy);
 #pragma unroll
                 for (int e = 0; e < P; ++e) {
-                    const float2 h = mul2(add2(fx[e], both(-mean)), both(rstd)), a = mul2(fy[e], fw[e]);
-                    fx[e] = fma2(a, both(rstd), fma2(h, kh, ka));
+                    const float2 h = mul2(add2(fx[e], both(-mean)), both(rstd));
+                    fx[e] = mul2(fma2(fy[e], fw[e], fma2(h, kh, ka)), both(rstd));
                 }
                 at.store(dx, j, pack<T, G>(fx));
             }
