@@ -113,6 +113,13 @@ void refuse_second_order(const char* what) {
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its backward pass has no gradient");
 }
 
+// A tangent (forward-mode differentiation) does not show in requires_grad, and an
+// output without one reads as a derivative of zero.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 at::DimVector with_last(const Tensor& x, int64_t n) {
     at::DimVector s(x.sizes().begin(), x.sizes().end());
     s.back() = n;
@@ -144,6 +151,7 @@ int64_t check_linear(const Tensor& x, const Tensor& w, const Tensor& bias, const
         TORCH_CHECK_VALUE(residual.sizes() == want, "residual must be ", at::IntArrayRef(want), ", got ",
                           residual.sizes());
     }
+    refuse_tangents("dense_linear", {&x, &w, &bias, &residual, &gate});
     return gate.defined() ? sample_rows("gate", gate.sizes(), x, n) : x.numel() / k;
 }
 
@@ -200,6 +208,7 @@ LinearGrads linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, 
         TORCH_CHECK_VALUE(!t->defined() || (t == &preact ? t->scalar_type() == at::kFloat || t->scalar_type() == at::kHalf
                                                          : t->scalar_type() == dt),
                           name, " is ", t->scalar_type(), ", dy is ", dt);
+    refuse_tangents("dense_linear_backward", {&dy, &x, &w, &preact, &gate});
     const int64_t m = dy.numel() / n;
     const int64_t rows_per_gate = gate.defined() ? sample_rows("gate", gate.sizes(), dy, n) : m;
     check_devices(dy, {&x, &w, &preact, &gate});
@@ -289,6 +298,7 @@ int64_t check_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps
     TORCH_CHECK_VALUE(!w.defined() || !b.defined() || (w.scalar_type() == b.scalar_type() && w.sizes() == b.sizes()),
                       "the two vectors must agree, got ", w.scalar_type(), " ", w.sizes(), " and ", b.scalar_type(), " ",
                       b.sizes());
+    refuse_tangents("layer_norm", {&x, &w, &b});
     const Tensor& v = w.defined() ? w : b;
     if (!v.defined()) return x.numel() / x.size(-1);
     TORCH_CHECK_VALUE(v.scalar_type() == dt || v.scalar_type() == at::kFloat, "the vectors must be ", dt,
@@ -344,6 +354,7 @@ NormGrads norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, cons
         TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->numel() == m, name, " must hold ", m,
                           " float32 values, got ", t->scalar_type(), " ", t->sizes());
     TORCH_CHECK_VALUE(vec_type == dt || vec_type == at::kFloat, "the vectors must be ", dt, " or float32, got ", vec_type);
+    refuse_tangents("layer_norm_backward", {&dy, &x, &w, &mean, &rstd});
     const int64_t rows_per_vec = sample_rows("the vectors", vec_shape, x, d);
     check_devices(dy, {&x, &w, &mean, &rstd});
     at::AutoDispatchBelowAutograd below;

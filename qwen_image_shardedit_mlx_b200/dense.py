@@ -10,8 +10,9 @@ The trainable twins of what the q6 block computes around its packed weights:
   fp16 or fp32 rows of any width.
 
 Both differentiate through ``torch.autograd`` and have functional forms
-(``*_forward`` / ``*_backward``) that launch the same kernels without it.  The
-functional forms may be captured in a CUDA graph.  A differentiable call under
+(``*_forward`` / ``*_backward``) that launch the same kernels without it.  Inputs
+with a forward-mode tangent are refused.  The functional forms may be captured in a
+CUDA graph.  A differentiable call under
 capture, and the backward pass of an earlier one, are refused: autograd would
 run parts of it on the streams that it recorded for the leaves, outside the
 capture.

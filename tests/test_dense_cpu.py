@@ -199,3 +199,42 @@ def test_no_samples_with_a_vector_each():
         dense.layer_norm_modulate(t(0, 4, 8), t(0, 8), t(0, 8))
     with pytest.raises(ValueError, match="samples"):
         dense.dense_linear(t(2, 4, 8), t(6, 8), gate=t(0, 6))
+
+
+def test_forward_mode_tangents_are_refused():
+    """Without a derivative of its own a call must not drop a tangent: torch would read it as zero."""
+    fw = torch.autograd.forward_ad
+
+    def refused(f):
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f()
+
+    x, w, b, r, g = t(4, 8), t(6, 8), t(6), t(4, 6), t(6)
+    with fw.dual_level():
+        for i in range(5):
+            for leaf in (False, True):  # with and without a gradient beside the tangent
+                a = [v.clone().requires_grad_(leaf) for v in (x, w, b, r, g)]
+                a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+                refused(lambda: dense.dense_linear(a[0], a[1], a[2], residual=a[3], gate=a[4]))
+                with torch.no_grad():
+                    refused(lambda: dense.dense_linear(a[0], a[1], a[2], residual=a[3], gate=a[4]))
+            refused(lambda: dense.dense_linear_forward(a[0], a[1], a[2], residual=a[3], gate=a[4]))
+        dy, z = t(4, 6), t(4, 6, dtype=torch.float16)
+        for i in range(5):
+            a = [v.clone() for v in (dy, x, w, z, g)]
+            a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+            refused(lambda: dense.dense_linear_backward(*a[:3], preact=a[3], gate=a[4]))
+        for i in range(3):
+            for leaf in (False, True):
+                a = [v.clone().requires_grad_(leaf) for v in (x, t(8), t(8))]
+                a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+                refused(lambda: dense.layer_norm(*a))
+                refused(lambda: dense.layer_norm_modulate(*a))
+            refused(lambda: dense.layer_norm_forward(*a))
+            refused(lambda: dense.layer_norm_modulate_forward(*a))
+        stats = torch.zeros(4)
+        for i in range(5):
+            a = [v.clone() for v in (x, x, t(8), stats, stats)]
+            a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+            refused(lambda: dense.layer_norm_backward(*a))
+            refused(lambda: dense.layer_norm_modulate_backward(*a))
