@@ -24,7 +24,8 @@
 // loads of bias, gate and residual and 16-byte stores.  Layouts that do not
 // allow that (odd widths, odd addresses) take one column per lane instead.
 //
-// Every mbarrier wait is bounded (q6_ptx.cuh).
+// Every mbarrier wait is bounded (q6_ptx.cuh) and begins after the previous kernel's
+// end, so that its limit covers this kernel's own pipeline alone.
 #pragma once
 
 #include <cuda.h>
@@ -615,6 +616,8 @@ __global__ void __launch_bounds__(kDenseThreads, 1)
         // The whole warp walks the loop so that the operands stay warp-uniform;
         // one elected lane issues a stage's MMAs and their commit.
         if (leader) {
+            // before the first timed wait: the previous kernel may run for longer than its limit
+            pdl_wait();
             const uint32_t idesc = (1u << 4) | ((p.half ? 0u : 1u) << 7) | ((p.half ? 0u : 1u) << 10) |
                                    ((kPT ? 1u : 0u) << 15) | ((kQT ? 1u : 0u) << 16) |
                                    (static_cast<uint32_t>(CT >> 3) << 17) | (static_cast<uint32_t>(kTileC >> 4) << 24);
