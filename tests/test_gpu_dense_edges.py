@@ -6,8 +6,10 @@ from __future__ import annotations
 import pytest
 import torch
 
-from qwen_image_shardedit_mlx_b200 import dense, ops
-from test_gpu_dense import DT, check_norm, rand
+import bounds
+from bounds import B
+from qwen_image_shardedit_mlx_b200 import _lib, dense, ops
+from test_gpu_dense import DT, check_norm, rand, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +71,127 @@ def test_product_behind_a_kernel_of_several_seconds():
         assert ops.device_error() == 0
         assert torch.equal(got, want)
         assert (db.float() > 0).all()
+
+
+class Guarded:
+    """Buffers carved out of one filled allocation: what lies between them must stay."""
+
+    FILL, GAP = 0xA5, 4096
+
+    def __init__(self, nbytes):
+        self.bytes = torch.full((nbytes,), self.FILL, dtype=torch.uint8, device="cuda")
+        self.at, self.parts = self.GAP, []
+
+    def take(self, nbytes, shift=0):
+        """Address of ``nbytes`` bytes, ``shift`` past a multiple of 256."""
+        start = self.at + (-(self.bytes.data_ptr() + self.at)) % 256 + shift
+        self.at = start + nbytes + self.GAP
+        assert self.at <= self.bytes.numel()
+        self.parts.append((start, nbytes))
+        return self.bytes.data_ptr() + start
+
+    def value(self, address, like):
+        """The buffer at ``address`` as a tensor of ``like``'s shape and type."""
+        start = address - self.bytes.data_ptr()
+        return self.bytes[start:start + like.numel() * like.element_size()].clone().view(like.dtype).reshape(like.shape)
+
+    def check(self):
+        outside = torch.ones_like(self.bytes, dtype=torch.bool)
+        for start, nbytes in self.parts:
+            outside[start:start + nbytes] = False
+        assert (self.bytes[outside] == self.FILL).all()
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+# few rows, one and two row tiles; ragged tiles; split sums; operands that are copied
+# first; single rows and columns
+GUARD_LINEAR = [(1, 264, 72), (7, 133, 57), (13, 520, 24), (16, 1031, 1), (17, 72, 40), (45, 264, 136), (150, 707, 773),
+                (300, 2056, 1032), (96, 4096, 131), (257, 8, 393), (515, 1, 9), (33, 63, 2050)]
+
+
+@pytest.mark.parametrize("m,k,n", GUARD_LINEAR)
+@pytest.mark.parametrize("shift", [0, 2])
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_writes_nothing_beside_its_buffers(m, k, n, shift, gated):
+    lib, dtype = _lib.lib(), torch.bfloat16
+    x, w, b, dy = (rand(s, dtype, i, std) for i, (s, std) in enumerate(
+        (((m, k), 1.0), ((n, k), k ** -0.5), ((n,), 0.5), ((m, n), 1.0))))
+    gates = 3 if gated and m % 3 == 0 else 1
+    gate = rand((gates, n), dtype, 5) if gated else None
+    xs = x.reshape(gates, -1, k)
+    y, z = dense.dense_linear_forward(xs, w, b, activation="gelu_tanh", gate=gate, save_preact=True)
+    outputs = ("x", "weight", "bias", "gate")[:4 if gated else 3]
+    want = dense.dense_linear_backward(dy.reshape(gates, -1, n), xs, w, preact=z, activation="gelu_tanh", gate=gate,
+                                       outputs=outputs)
+    pack = sum(bit for bit, odd in ((_lib.Q6_PACK_X, k % 8), (_lib.Q6_PACK_W, k % 8), (_lib.Q6_PACK_DY, n % 8)) if odd)
+    gate_args = (gate.data_ptr() if gated else None, n, m // gates)
+    zt = _lib.Q6_DTYPE_F32 if gated else _lib.Q6_DTYPE_F16
+
+    nbytes = lib.q6_dense_linear_workspace_bytes(m, n, k, pack)
+    g = Guarded(nbytes + 8 * m * n + (1 << 16))
+    py, pz, ws = g.take(2 * m * n, shift), g.take(z.element_size() * m * n, 2 * shift), g.take(nbytes)
+    status = lib.q6_dense_linear(x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), *gate_args, None, 0, py, pz, zt, m, n, k,
+                                 _lib.Q6_DTYPE_BF16, _lib.Q6_ACT_GELU_TANH, ws if nbytes else None, nbytes, stream())
+    assert status == 0
+    g.check()
+    assert torch.equal(g.value(py, y), y) and torch.equal(g.value(pz, z), z)
+
+    flags = _lib.Q6_GRAD_X | _lib.Q6_GRAD_W | _lib.Q6_GRAD_BIAS | (_lib.Q6_GRAD_GATE if gated else 0)
+    nbytes = lib.q6_dense_linear_grad_workspace_bytes(m, n, k, m // gates, _lib.Q6_ACT_GELU_TANH, int(gated), flags, pack)
+    g = Guarded(nbytes + 2 * (m * k + n * k + 4 * n) + (1 << 16))
+    pdx, pdw, pdb = g.take(2 * m * k, shift), g.take(2 * n * k, shift), g.take(2 * n, shift)
+    pdg = g.take(2 * n * gates, shift) if gated else None
+    ws = g.take(nbytes)
+    status = lib.q6_dense_linear_grad(dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), k, z.data_ptr(), zt, *gate_args, pdx,
+                                      pdw, pdb, pdg, m, n, k, _lib.Q6_DTYPE_BF16, _lib.Q6_ACT_GELU_TANH, ws, nbytes,
+                                      stream())
+    assert status == 0
+    g.check()
+    assert torch.equal(g.value(pdx, x), want.x.reshape(m, k)) and torch.equal(g.value(pdw, w), want.weight)
+    assert torch.equal(g.value(pdb, b), want.bias)
+    if gated:
+        assert torch.equal(g.value(pdg, gate), want.gate)
+
+
+@pytest.mark.parametrize("vecs,rows,d", [(1, 1, 1), (1, 5, 3), (2, 7, 33), (1, 37, 64), (3, 50, 100), (2, 40, 256),
+                                         (1, 17, 1001), (2, 33, 1536), (1, 301, 128), (1, 5, 8200), (1, 2, 33001)])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_norm_writes_nothing_beside_its_buffers(vecs, rows, d, shift, dtype):
+    lib, dt, m = _lib.lib(), DT[dtype], vecs * rows
+    code = {"bf16": _lib.Q6_DTYPE_BF16, "fp32": _lib.Q6_DTYPE_F32}[dtype]
+    size = dt.itemsize
+    x, dy = rand((vecs, rows, d), dt, 1, 2.0), rand((vecs, rows, d), dt, 2)
+    scale, bias = rand((vecs, d), dt, 3, 0.3), rand((vecs, d), dt, 4, 0.3)
+    y, mean, rstd = dense.layer_norm_modulate_forward(x, bias, scale)
+    g = Guarded(m * d * size + 8 * m + (1 << 16))
+    py, pm, pr = g.take(m * d * size, shift * size), g.take(4 * m, shift * 4), g.take(4 * m)
+    status = lib.q6_layer_norm(x.data_ptr(), d, scale.data_ptr(), bias.data_ptr(), d, rows, py, pm, pr, m, d, 1e-6, code,
+                               code, _lib.Q6_NORM_ONE_PLUS, stream())
+    assert status == 0
+    g.check()
+    # an odd address takes another kernel, with sums in another order: each within its own bound
+    bx, bw, bb = B(x.reshape(m, d)), B(spread(scale.double() + 1.0, m), 2.0 ** -22), B(spread(bias, m))
+    ry, xh, rs = bounds.norm(bx, bw, bb, 1e-6, dt)
+    for p, ref, bound in ((py, y, ry), (pm, mean, bx.mean()), (pr, rstd, rs)):
+        bound.check(g.value(p, ref).reshape(bound.v.shape), "forward")
+        assert shift or torch.equal(g.value(p, ref), ref)
+
+    want = dense.layer_norm_modulate_backward(dy, x, scale, mean, rstd)
+    flags = _lib.Q6_GRAD_W | _lib.Q6_GRAD_BIAS
+    nbytes = lib.q6_layer_norm_grad_workspace_bytes(m, d, rows, code, flags)
+    g = Guarded(m * d * size + 2 * vecs * d * size + nbytes + (1 << 16))
+    pdx, pdw, pdb = (g.take(v * d * size, shift * size) for v in (m, vecs, vecs))
+    ws = g.take(nbytes)
+    status = lib.q6_layer_norm_grad(dy.data_ptr(), d, x.data_ptr(), d, scale.data_ptr(), d, rows, mean.data_ptr(),
+                                    rstd.data_ptr(), pdx, pdw, pdb, m, d, code, code, _lib.Q6_NORM_ONE_PLUS,
+                                    ws if nbytes else None, nbytes, stream())
+    assert status == 0
+    g.check()
+    dx, dw, db = bounds.norm_grads(B(dy.reshape(m, d)), xh, rs, bw, dt, dt, vecs)
+    for p, ref, bound in ((pdx, want.x, dx), (pdw, want.weight, dw), (pdb, want.bias, db)):
+        bound.check(g.value(p, ref).reshape(bound.v.shape), "backward")
+        assert shift or torch.equal(g.value(p, ref), ref)
