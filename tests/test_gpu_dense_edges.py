@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import bounds
 from bounds import B
@@ -195,3 +196,99 @@ def test_norm_writes_nothing_beside_its_buffers(vecs, rows, d, shift, dtype):
     for p, ref, bound in ((pdx, want.x, dx), (pdw, want.weight, dw), (pdb, want.bias, db)):
         bound.check(g.value(p, ref).reshape(bound.v.shape), "backward")
         assert shift or torch.equal(g.value(p, ref), ref)
+
+
+@pytest.mark.parametrize("off", [0, 8, 5])
+def test_rows_of_every_operand_far_apart(off):
+    """Operands whose rows pass 2^31 elements, through the tensor maps, the aligned copies
+    (odd addresses), the strided residual and gates, and every gradient."""
+
+    base = torch.zeros((2200, 1 << 20), dtype=torch.bfloat16, device="cuda")
+
+    def far(rows, cols, at, seed, std=1.0):
+        step = 2199 // (rows - 1)
+        assert (rows - 1) * step << 20 > 1 << 31
+        v = base[:(rows - 1) * step + 1:step, at + off:at + off + cols]
+        v.copy_(rand((rows, cols), torch.bfloat16, seed, std))
+        return v
+
+    m, k, n = 21, 264, 136
+    args = [far(m, k, 0, 1), far(n, k, 1000, 2, 0.1), far(m, n, 2000, 3), far(m, n, 3000, 4), far(m, n, 4000, 5)]
+    near = [v.contiguous() for v in args]
+
+    def passes(x, w, r, dy, g):
+        out = []
+        for act, gate in (("gelu_tanh", None), ("silu", g)):  # one vector, and one per row
+            y, z = dense.dense_linear_forward(x, w, activation=act, residual=r, gate=gate, save_preact=True)
+            outputs = ("x", "weight", "bias") + (("gate",) if gate is not None else ())
+            out += [y, z, *dense.dense_linear_backward(dy, x, w, preact=z, activation=act, gate=gate, outputs=outputs)]
+        out += dense.dense_linear_backward(dy, x, w)  # dy itself is the products' operand
+        h, mean, rstd = dense.layer_norm_modulate_forward(r, g, dy)
+        return out + [h, mean, rstd, *dense.layer_norm_modulate_backward(dy, r, g, mean, rstd)]
+
+    got, want = passes(*args), passes(*near)
+    for a, b in zip(got, want):
+        assert (a is None) == (b is None)
+        if a is not None:
+            if off == 5 and a.shape == (m,):  # the norm's kernel without 16-byte accesses sums in another order
+                assert (a - b).abs().max() <= n * 2.0 ** -23 * b.abs().max() * 4
+            elif off == 5 and a.dtype == torch.bfloat16:
+                assert (a.double() - b.double()).abs().max() <= 2.0 ** -7 * b.double().abs().max()
+            else:
+                assert torch.equal(a, b)
+    if off == 5:
+        for a, b in zip(got[:-6], want[:-6]):
+            assert (a is None and b is None) or torch.equal(a, b)
+
+
+def test_calls_from_several_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            x, w, b = (rand(s, torch.bfloat16, i + j) for j, s in enumerate(((3, 60 + i, 136), (200, 136), (136,))))
+            leaves = [v.requires_grad_(True) for v in (x, w, b)]
+            out = []
+            for _ in range(8):
+                y = dense.dense_linear(dense.layer_norm(x, b, b), w, activation="silu")
+                out.append([y.detach(), *torch.autograd.grad(y.float().sum(), leaves)])
+            torch.cuda.current_stream().synchronize()
+        return out
+
+    with ThreadPoolExecutor(4) as pool:
+        together = list(pool.map(work, range(8)))
+    for i, runs in enumerate(together):
+        alone = work(i)[0]
+        for run in runs:
+            assert all(torch.equal(a, b) for a, b in zip(run, alone))
+
+
+def test_saved_tensor_hooks_and_recomputation():
+    x, w, b, gate = (rand(s, torch.bfloat16, i) for i, s in enumerate(((2, 40, 72), (136, 72), (136,), (2, 136))))
+    leaves = [v.requires_grad_(True) for v in (x, w, b, gate)]
+    dy = rand((2, 40, 136), torch.bfloat16, 9)
+
+    def half(x, w, b, gate):
+        return dense.dense_linear(dense.layer_norm(x), w, b, activation="gelu_tanh", gate=gate)
+
+    want = torch.autograd.grad(half(*leaves), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = half(*leaves)
+    kept = torch.autograd.grad(y, leaves, dy)
+    again = torch.autograd.grad(torch.utils.checkpoint.checkpoint(half, *leaves, use_reentrant=False), leaves, dy)
+    for a, b_, c in zip(want, kept, again):
+        assert torch.equal(a, b_) and torch.equal(a, c)
+
+
+def test_function_transforms_are_refused():
+    """torch.func wraps tensors: a call must not compute without the wrapper's derivative or batch."""
+
+    x, w = rand((4, 16), torch.bfloat16, 1), rand((8, 16), torch.bfloat16, 2)
+    for f in (lambda v: dense.dense_linear(v, w).float().sum(), lambda v: dense.layer_norm(v).float().sum()):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(x)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x)
+    assert dense.dense_linear(x, w).shape == (4, 8)  # and nothing of it lingers
