@@ -13,10 +13,12 @@ against that library.
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -26,6 +28,7 @@ CSRC = PKG / "csrc"
 BUILD = CSRC / "_build"
 LIB = PKG / "libq6b200.so"
 EXT = PKG / "_q6torch.so"
+EXT_SOURCE = CSRC / "q6_torch.cpp"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -91,15 +94,32 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     if force or cmds or _needs(LIB, objs):
         link = [nvcc(), *ARCH, "-shared", "-cudart", "static", *[str(o) for o in objs], "-o", str(LIB)]
         run(link)
-    ext = CSRC / "q6_torch.cpp"
-    if force or _needs(EXT, [ext, INCLUDE / "q6_b200.h", LIB]):
-        run(_torch_extension_command(ext))
+    if force or _extension_stale():
+        run(_torch_extension_command(EXT_SOURCE))
+        _stamp().write_text(_torch_abi())
     return LIB
 
 
-def _torch_extension_command(src: Path) -> list[str]:
-    import sysconfig
+def _stamp() -> Path:
+    return BUILD / (EXT.stem + ".abi")
 
+
+def _torch_abi() -> str:
+    """What the extension module is bound to besides its sources."""
+
+    return f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _extension_stale() -> bool:
+    """Older than its sources, or built against another torch or Python: it would
+    not load, whatever the file times say."""
+
+    if _needs(EXT, [EXT_SOURCE, INCLUDE / "q6_b200.h", LIB]):
+        return True
+    return not _stamp().exists() or _stamp().read_text() != _torch_abi()
+
+
+def _torch_extension_command(src: Path) -> list[str]:
     import torch
     from torch.utils import cpp_extension
 
