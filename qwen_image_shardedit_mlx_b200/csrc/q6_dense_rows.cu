@@ -206,10 +206,16 @@ cudaError_t launch_typed(const RowsParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Up to eight rows always.  To sixteen, x is as large as a CTA's part of the
-// weight, and an SM takes in both: the tcgen05 path, which reads x once per 128
-// rows of W, wins where the sum is long or the weight large.  Sixteen rows of bf16,
-// here against there: 768 -> 768 2.8 / 5.7 us, 3072 -> 3072 7.9 / 9.5, 4096 -> 4096
+// Here against the tcgen05 path, bf16, in us.
+// Up to eight rows: one row 1024 -> 1024 2.9 / 6.6, 3072 -> 64 3.4 / 7.2, 12288 -> 64
+// 7.4 / 9.1, 12288 -> 3072 15.2 / 19.0, 3072 -> 18432 20.0 / 21.5; eight rows 3.1 / 6.7,
+// 3.5 / 7.2, 7.5 / 9.4, 16.9 / 19.7, 21.1 / 21.8; nearest 12288 -> 1024, 11.3 / 11.8 and
+// 12.6 / 12.1.  The sum is not split over CTAs, so a longer one with few outputs
+// takes longer here: one row 18432 -> 128 12.7 / 11.2, 49152 -> 64 27.7 / 15.6.  The rule
+// has no case for those: no layer here sums over more than 12288.
+// To sixteen, x is as large as a CTA's part of the weight, and an SM takes in both:
+// the tcgen05 path, which reads x once per 128 rows of W, wins where the sum is long
+// or the weight large: 768 -> 768 2.8 / 5.7, 3072 -> 3072 7.9 / 9.5, 4096 -> 4096
 // 10.0 / 12.1, 6144 -> 3072 12.6 / 13.5, 3072 -> 9216 13.3 / 15.3; 3072 -> 12288
 // 17.7 / 17.1, 9216 -> 3072 17.5 / 16.4, 12288 -> 1024 17.5 / 11.8.
 bool dense_few_rows(int64_t R, int64_t C, int64_t L) {

@@ -74,24 +74,6 @@ __device__ __forceinline__ float2 warp_sum2(float2 v) {
     return odd ? make_float2(other, s) : make_float2(s, other);
 }
 
-// The same for two rows' pairs: two exchanges leave one value per lane, so four
-// sums cost nine shuffles.
-__device__ __forceinline__ void warp_sum2(float2& a, float2& b) {
-    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
-    float s0 = odd ? a.y : a.x, s1 = odd ? b.y : b.x;
-    s0 += __shfl_xor_sync(0xffffffffu, odd ? a.x : a.y, 1);
-    s1 += __shfl_xor_sync(0xffffffffu, odd ? b.x : b.y, 1);
-    float s = high ? s1 : s0;
-    s += __shfl_xor_sync(0xffffffffu, high ? s0 : s1, 2);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    // lane l of every four holds value l: a.x, a.y, b.x, b.y
-    a.x = __shfl_sync(0xffffffffu, s, 0);
-    a.y = __shfl_sync(0xffffffffu, s, 1);
-    b.x = __shfl_sync(0xffffffffu, s, 2);
-    b.y = __shfl_sync(0xffffffffu, s, 3);
-}
-
 // Sum over each run of L lanes.
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
@@ -358,7 +340,7 @@ __global__ void __launch_bounds__(32 * CW * grad_row_lanes(CW), 1)
     __shared__ float4 stats[2][TR];  // -mean, rstd and, with a warp per row in phase A, c and k
     __shared__ __align__(8) uint64_t full[kGradMaxStages];
     __shared__ int abort_word;
-    extern __shared__ __align__(128) uint8_t smem[];  // the ring, the factors [D]; in the end the column sums [2][D]
+    extern __shared__ __align__(128) uint8_t smem[];  // the ring, the factors [D]; in the end the column sums (finish_bytes)
     pdl_launch_dependents();
     const int D = static_cast<int>(p.D), groups = D / G;
     const uint32_t row_bytes = static_cast<uint32_t>(D * sizeof(T)), tile_bytes = TR * 2 * row_bytes;
@@ -554,7 +536,7 @@ __global__ void __launch_bounds__(32 * CW * (CW < 16 ? 16 / CW : 1), 1)
     constexpr int G = 16 / sizeof(T), P = G / 2, RL = CW < 16 ? 16 / CW : 1, kThreads = 32 * CW;
     static_assert(RL < 16 || CW == 1, "named barriers");
     __shared__ __align__(16) float2 parts[2][RL][CW];
-    extern __shared__ __align__(128) uint8_t smem[];  // the column sums [2][D]
+    extern __shared__ __align__(128) uint8_t smem[];  // the column sums (finish_bytes)
     pdl_launch_dependents();
     pdl_wait();
     const int group = threadIdx.x / kThreads;
