@@ -54,6 +54,11 @@ void* mutable_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() :
 Tensor of(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 OptTensor optional_of(Tensor t) { return t.defined() ? OptTensor(std::move(t)) : std::nullopt; }
 
+// `t` with its values as they lie in memory: a tensor may stand for the negative of
+// what it stores (the imaginary part of a conjugate).
+Tensor stored(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor contiguous(const Tensor& t) { return t.defined() ? stored(t).contiguous() : t; }
+
 // `t` as rows of `width` with contiguous columns and the stride between rows (a
 // copy only where the layout does not allow that).
 struct Rows {
@@ -61,7 +66,8 @@ struct Rows {
     int64_t ld = 0;
 };
 
-Rows rows_of(const Tensor& t, int64_t width) {
+Rows rows_of(const Tensor& given, int64_t width) {
+    const Tensor t = stored(given);
     if (!t.defined() || t.is_contiguous()) return {t, width};
     Tensor t2 = t.reshape({-1, width});
     const int64_t rows = t2.size(0);
@@ -169,7 +175,7 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
     Tensor z = save_preact ? like(x, shape, zt) : Tensor();
     if (m == 0) return {y, z};
     const Rows rx = rows_of(x, k), rw = rows_of(w, k), rr = rows_of(residual, n), rg = rows_of(gate, n);
-    const Tensor b = bias.defined() ? bias.contiguous() : bias;
+    const Tensor b = contiguous(bias);
     const size_t bytes =
         q6_dense_linear_workspace_bytes(m, n, k, pack_bit(rx, Q6_PACK_X) | pack_bit(rw, Q6_PACK_W));
     const Tensor ws = workspace(bytes, x);
@@ -224,7 +230,7 @@ LinearGrads linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, 
     const Rows ry = rows_of(dy, n), rg = rows_of(gate, n);
     const Rows rx = (want & Q6_GRAD_W) ? rows_of(x, k) : Rows{Tensor(), k};
     const Rows rw = (want & Q6_GRAD_X) ? rows_of(w, k) : Rows{Tensor(), k};
-    const Tensor z = preact.defined() ? preact.contiguous() : preact;
+    const Tensor z = contiguous(preact);
     const int pack = pack_bit(rx, Q6_PACK_X) | pack_bit(rw, Q6_PACK_W) | pack_bit(ry, Q6_PACK_DY);
     const size_t bytes = q6_dense_linear_grad_workspace_bytes(m, n, k, rows_per_gate, activation, gate.defined(), want,
                                                               pack);
@@ -366,7 +372,7 @@ NormGrads norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, cons
     if (want_b) g.bias = like(x, vec_shape, vec_type, none);
     if (none || !(want_x || want_w || want_b)) return g;
     const Rows rx = rows_of(x, d), ry = rows_of(dy, d), rw = rows_of(w, d);
-    const Tensor mu = mean.contiguous(), rs = rstd.contiguous();
+    const Tensor mu = contiguous(mean), rs = contiguous(rstd);
     const int code = dtype_code(dt), bits = (want_w ? Q6_GRAD_W : 0) | (want_b ? Q6_GRAD_BIAS : 0);
     const size_t bytes = bits ? q6_layer_norm_grad_workspace_bytes(m, d, rows_per_vec, code, bits) : 0;
     const Tensor ws = workspace(bytes, x);

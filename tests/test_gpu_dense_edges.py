@@ -292,3 +292,24 @@ def test_function_transforms_are_refused():
         with pytest.raises(RuntimeError):
             torch.func.vmap(f)(x)
     assert dense.dense_linear(x, w).shape == (4, 8)  # and nothing of it lingers
+
+
+def test_tensors_that_stand_for_their_negative():
+    # the imaginary part of a conjugate is a view with a sign to apply; one column of it needs no copy
+    both = torch.view_as_complex(rand((6, 1, 2), torch.float32, 1)).conj()
+    x, plain = both.imag, both.imag.resolve_neg()
+    assert x.is_neg() and not plain.is_neg()
+    zeros, ones = torch.zeros((6, 1), device="cuda"), torch.ones((6, 1), device="cuda")
+    b = rand((1,), torch.float32, 2)
+    for call in (lambda v: dense.layer_norm_forward(v, b, b), lambda v: dense.layer_norm_modulate_forward(ones, v, v),
+                 lambda v: dense.layer_norm_backward(v, ones, None, zeros[:, 0], ones[:, 0]),
+                 lambda v: dense.layer_norm_backward(ones, ones, None, v, v)):
+        for got, want in zip(call(x), call(plain)):
+            assert (got is None and want is None) or torch.equal(got, want)
+    w, flipped = rand((24, 16), torch.bfloat16, 3), torch._neg_view(rand((24, 16), torch.bfloat16, 3))
+    a = rand((40, 16), torch.bfloat16, 4)
+    assert torch.equal(dense.dense_linear(a, flipped, flipped[:, 0]), dense.dense_linear(a, -w, -w[:, 0]))
+    dy, z = rand((40, 24), torch.bfloat16, 5), rand((40, 24), torch.float32, 6)
+    for got, want in zip(dense.dense_linear_backward(torch._neg_view(dy), a, w, preact=torch._neg_view(z), activation="silu"),
+                         dense.dense_linear_backward(-dy, a, w, preact=-z, activation="silu")):
+        assert (got is None and want is None) or torch.equal(got, want)
