@@ -130,7 +130,8 @@ def dense_linear_backward(
     may be None without "weight", ``weight`` may be None without "x".
     ``preact`` is the forward's, needed with an activation or for "gate".  The
     weight's and the x gradient multiply the gradient of the pre-activation
-    rounded to the tensors' dtype; all sums are held in fp32.
+    rounded to the tensors' dtype (in fp16 with that type's range: beyond 65504 it is
+    infinite); all sums are held in fp32.
     """
 
     want = 0
