@@ -328,6 +328,8 @@ int q6_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bi
     p.M = M;
     p.D = D;
     p.eps = eps;
+    p.inv = 1.0f / static_cast<float>(D);
+    p.inv_rest = static_cast<float>(1.0 / static_cast<double>(D) - static_cast<double>(p.inv));
     p.one = (flags & Q6_NORM_ONE_PLUS) ? 1.0f : 0.0f;
     return with_types(dtype, vec_dtype, [&](auto t, auto v) {
         return run_forward<decltype(t), decltype(v)>(p, reinterpret_cast<cudaStream_t>(stream));

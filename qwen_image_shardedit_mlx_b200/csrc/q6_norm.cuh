@@ -57,6 +57,7 @@ struct NormParams {
     int64_t strip_rows, strips_per_vec;
     unsigned col_blocks;
     unsigned vecs;  // forward: vectors, where they are the grid's second axis (else 0)
+    float inv, inv_rest;  // forward: 1 / D rounded, and what the rounding left
 };
 
 
@@ -72,6 +73,15 @@ __device__ __forceinline__ float2 warp_sum2(float2 v) {
     for (int o = 2; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const float other = __shfl_xor_sync(0xffffffffu, s, 1);
     return odd ? make_float2(other, s) : make_float2(s, other);
+}
+
+// The mean of a row from its sum, rounded once: sum (inv + inv_rest) carries 1 / D to 47
+// bits.  sum * inv alone may be a step off; for a constant row (padding) the variance
+// takes that step for the row's spread, and 1920 values of -65504 came out as +-1.
+// An infinite sum stays so.  (A division costs registers: 5000 x 12288 40.6 -> 52.9 us.)
+__device__ __forceinline__ float norm_mean(float sum, const NormParams& p) {
+    const float rest = __fmul_rn(sum, p.inv_rest);
+    return __fmaf_rn(sum, p.inv, isinf(sum) ? 0.0f : rest);
 }
 
 // Sum over each run of L lanes.
@@ -184,7 +194,6 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormP
     Group<T, G> in[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) in[j] = at.load(x, j);
-    const float inv = 1.0f / static_cast<float>(at.D);
     for (;; local += step, warp_row += step) {
         const int64_t row = row0 + row_of(local);
         const bool more = warp_row + step < limit, ours = L == 32 || local < limit;
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormP
                 for (int i = 0; i < G / 2; ++i) s = add2(s, c[j][i]);
             }
         }
-        const float mean = row_sum(s.x + s.y, 0) * inv;
+        const float mean = norm_mean(row_sum(s.x + s.y, 0), p);
         float2 q = both(0.0f);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -230,7 +239,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) norm_kernel(const NormP
                 }
             }
         }
-        const float rstd = rsqrtf(row_sum(q.x + q.y, 1) * inv + p.eps);
+        const float rstd = rsqrtf(row_sum(q.x + q.y, 1) * p.inv + p.eps);
         if (p.mean && at.t == 0 && ours) {
             p.mean[row] = mean;
             p.rstd[row] = rstd;

@@ -313,3 +313,26 @@ def test_tensors_that_stand_for_their_negative():
     for got, want in zip(dense.dense_linear_backward(torch._neg_view(dy), a, w, preact=torch._neg_view(z), activation="silu"),
                          dense.dense_linear_backward(-dy, a, w, preact=-z, activation="silu")):
         assert (got is None and want is None) or torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [1, 3, 7, 13, 14, 56, 61, 120, 224, 480, 960, 1001, 1920, 3000, 3072, 4097, 7680, 8192])
+def test_norm_constant_rows_have_no_spread(dtype, d):
+    """A row of one value (padding, a fill with the type's lowest value): its sums are exact
+    in fp32 (at most 11 bits a value, 2^13 of them), so its mean is that value and its
+    output the bias alone."""
+
+    fi = torch.finfo(DT[dtype])
+    big = 2.0 ** 60 if dtype == "bf16" else fi.max
+    values = [0.0, 1.0, -3.0, 1.0 + fi.eps, 255.0, -1000.0, 2.0 ** 15 * (2 - fi.eps), -big, big / 3, big / 1.7]
+    x = torch.tensor(values, dtype=DT[dtype], device="cuda")[:, None].expand(-1, d).contiguous()
+    w, b = rand((d,), DT[dtype], 1), rand((d,), DT[dtype], 2)
+    y, mean, rstd = dense.layer_norm_forward(x, w, b)
+    assert torch.equal(mean, x[:, 0].float())
+    assert torch.equal(y, b.expand_as(y))
+    assert ((rstd - 1000.0).abs() <= 1e-3).all()
+    y, mean, _ = dense.layer_norm_modulate_forward(x[:, None], b, w)
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y[:, 0], b.expand_as(x))
+    for value in (float("inf"), float("-inf")):  # an infinite mean stays what it is
+        _, mean, _ = dense.layer_norm_forward(torch.full((2, d), value, dtype=DT[dtype], device="cuda"))
+        assert (mean == value).all()
