@@ -329,7 +329,8 @@ Q6_API size_t q6_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, i
  *   dx = dz @ W [M, K],  dw = dz^T @ x [N, K],  dbias = sum_m dz [N],
  *   dgate[s] = sum over the rows m of vector s of dy * act(z)   ([M / rows_per_gate, N]),
  * each written only if its pointer is non-null, dense, in dtype (sums in fp32;
- * dz is rounded to dtype as the operand of the two products).  The residual's
+ * dz is rounded to dtype as the operand of the two products).  No output may overlap
+ * an input or another output.  The residual's
  * gradient is dy itself.  preact is the forward's (may be null without an
  * activation and without dgate).  x is read only for dw, W only for dx.
  */
@@ -353,6 +354,7 @@ Q6_API size_t q6_dense_linear_grad_workspace_bytes(int64_t M, int64_t N, int64_t
  *   Q6_NORM_ONE_PLUS the factor is 1 + weight (adaLN: weight = scale, bias = shift).
  *   mean, rstd (fp32 [M], nullable together) receive the row statistics.
  * x [M, D] (ldx), y [M, D] dense.  dtype: BF16, F16 or F32; statistics and sums in fp32.
+ * No output may overlap an input, here and in the gradients.
  */
 enum q6_norm_flags { Q6_NORM_ONE_PLUS = 1 };
 
