@@ -157,7 +157,7 @@ struct Columns {
 
 // Forward: W warps per row (one row per CTA), or L lanes (128 / L rows per CTA; a
 // row of 128 in a warp of its own left half its lanes idle: 165888 rows of bf16
-// 37.6 us, 20.4 so), N groups per thread.  N is at most four: a row's code runs
+// 37.6 us, 20.8 so), N groups per thread.  N is at most four: a row's code runs
 // once per row, and with twelve groups per lane (a warp per row of 3072) its
 // unrolled length ran out of the instruction cache: 31 us for 6912 rows of bf16
 // against 21 us with four.  The grid is one wave of CTAs that walk the rows, the
